@@ -142,6 +142,9 @@ def core():
         lib.ie_argmax.argtypes = [P, P, I, I, L, P]
         lib.ie_repetition_penalty.argtypes = [P, P, P, I, I, L, I, P]
         lib.ie_sample.argtypes = [P, P, P, I, I, L, P]
+        lib.ie_history_reset.argtypes = [P, P, P, I, I, I, P]
+        lib.ie_history_append.argtypes = [P] * 6 + [I] * 4 + [P]
+        lib.ie_adjust_logits.argtypes = [P, I] + [P] * 10 + [I, I, L, L, I, I, I, I, P]
         for name in ("ie_embed_gather", "ie_rmsnorm", "ie_residual_add", "ie_rope_kv_write", "ie_silu_mul",
                      "ie_attention_general", "ie_gemm_simt", "ie_argmax", "ie_repetition_penalty", "ie_sample",
                      "ie_layernorm", "ie_embed_bigram", "ie_add_bias", "ie_tanh", "ie_polynorm",
@@ -151,7 +154,8 @@ def core():
                      "ie_heads_gemm", "ie_diff_combine", "ie_gated_residual_add", "ie_scale_rows", "ie_glu_act",
                      "ie_mingru_scan", "ie_mingru_scan_hint", "ie_scale_add_sinusoid", "ie_add_row", "ie_token_shift",
                      "ie_gate_mul", "ie_qkv_prepare", "ie_talk_combine", "ie_mlstm_scan", "ie_mlstm_finish",
-                     "ie_mlstm_chunks", "ie_stream_norm", "ie_conv_qkv", "ie_relu2", "ie_softcap"):
+                     "ie_mlstm_chunks", "ie_stream_norm", "ie_conv_qkv", "ie_relu2", "ie_softcap",
+                     "ie_history_reset", "ie_history_append", "ie_adjust_logits"):
             getattr(lib, name).restype = c_int
         _core = lib
         _apply_check_limits()
@@ -1082,6 +1086,135 @@ def sample(logits: torch.Tensor, rows: torch.Tensor, out: torch.Tensor) -> None:
                             logits.stride(0), _stream()), "sample")
 
 
+# ------------------------------------------- a request's history, and the logits that it changes
+def _need(holds: bool, what: str, why: str) -> None:
+    if not holds:
+        raise KernelError(f"{what}: refused ({why})")
+
+
+def _here(what: str, **tensors: torch.Tensor | None) -> None:
+    """The tensors lie on the current device, whose stream the kernels go to."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if dev is None and t.is_cuda:
+            dev = torch._C._cuda_getDevice()
+        if not t.is_cuda or t.get_device() != dev:
+            raise KernelError(f"{what}: {name} is on {t.device}, kernels run on tensors of the current device")
+
+
+def _ints(t: torch.Tensor) -> bool:
+    return t.dtype is torch.int32 and t.is_contiguous()
+
+
+def _history(what: str, counts: torch.Tensor, seen: torch.Tensor) -> tuple[int, int]:
+    _need(counts.dim() == 2 and _ints(counts), what, "counts is a contiguous int32 [slots, vocab]")
+    n_slots, vocab = counts.shape
+    _need(seen.shape == (n_slots, -(-vocab // 32)) and _ints(seen), what, "seen is a contiguous int32 [slots, ceil(vocab / 32)]")
+    return n_slots, vocab
+
+
+def history_reset(counts: torch.Tensor, seen: torch.Tensor, slots: torch.Tensor) -> None:
+    """Forgets what the requests in ``slots`` (int32 [n]) have said: counts[slot] = 0, seen[slot] = 0.  A slot that is
+    negative, or beyond the table, is passed over.  ``counts`` int32 [slots, vocab]; ``seen`` int32 [slots, ceil(vocab / 32)],
+    bit t % 32 of word t / 32."""
+    n_slots, vocab = _history("history_reset", counts, seen)
+    _need(slots.dim() == 1 and _ints(slots), "history_reset", "slots is a contiguous int32 [n]")
+    _here("history_reset", counts=counts, seen=seen, slots=slots)
+    _check(core().ie_history_reset(counts.data_ptr(), seen.data_ptr(), slots.data_ptr(), slots.shape[0], n_slots, vocab, _stream()),
+           "history_reset")
+
+
+def history_append(counts: torch.Tensor, seen: torch.Tensor, tokens: torch.Tensor, slots: torch.Tensor,
+                   starts: torch.Tensor | None = None, n_prompt: torch.Tensor | None = None) -> None:
+    """Adds ``tokens`` (int32 [T]) to the histories of ``slots`` (int32 [R]).  Tokens ``starts[r] .. starts[r + 1]`` (int32 [R + 1],
+    ascending; None: one token a slot) belong to slot r, and the first ``n_prompt[r]`` of them (int32 [R]; None: none) to its prompt:
+    those set the bit in ``seen``; every other token also adds one to ``counts``.  A token outside the vocabulary, or of a slot that
+    is negative or beyond the table, is passed over.  Tokens and slots may come more than once."""
+    n_slots, vocab = _history("history_append", counts, seen)
+    n, r = tokens.shape[0], slots.shape[0]
+    _need(tokens.dim() == 1 and _ints(tokens) and slots.dim() == 1 and _ints(slots), "history_append",
+          "tokens and slots are contiguous int32 vectors")
+    _need(starts is not None or n == r, "history_append", "without starts there is one token a slot")
+    _need(starts is None or (starts.shape == (r + 1,) and _ints(starts)), "history_append", "starts is a contiguous int32 [slots + 1]")
+    _need(n_prompt is None or (n_prompt.shape == (r,) and _ints(n_prompt)), "history_append", "n_prompt is a contiguous int32 [slots]")
+    _here("history_append", counts=counts, seen=seen, tokens=tokens, slots=slots, starts=starts, n_prompt=n_prompt)
+    _check(core().ie_history_append(counts.data_ptr(), seen.data_ptr(), tokens.data_ptr(), slots.data_ptr(), _ptr(starts),
+                                    _ptr(n_prompt), n, r, n_slots, vocab, _stream()), "history_append")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices (rows of adjacent elements) share a byte."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    ea, eb = a.element_size(), b.element_size()
+    (na, wa), (nb, wb) = a.shape, b.shape
+    pa, pb, sa, sb = a.data_ptr(), b.data_ptr(), a.stride(0) * ea, b.stride(0) * eb
+    if pa + (na - 1) * sa + wa * ea <= pb or pb + (nb - 1) * sb + wb * eb <= pa:
+        return False
+    if sa == sb and sa > 0:                  # columns of one buffer, side by side
+        d = (pb - pa) % sa
+        return not (d >= wa * ea and sa - d >= wb * eb)
+    return True
+
+
+def adjust_logits(logits: torch.Tensor, out: torch.Tensor, slots: torch.Tensor | None = None,
+                  penalties: torch.Tensor | None = None, counts: torch.Tensor | None = None, seen: torch.Tensor | None = None,
+                  bias_start: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+                  bias_values: torch.Tensor | None = None, mask_rows: torch.Tensor | None = None,
+                  masks: torch.Tensor | None = None) -> None:
+    """out = logits (float32 or bfloat16 [n, vocab]) with each row's penalties, biases and mask, float32.  ``out`` may be ``logits``
+    itself; otherwise the two share no memory.
+
+    Penalties (all four or none): row i reads the history ``slots[i]`` (int32 [n]; outside the table: none) and
+    ``penalties[i]`` = (repetition, presence, frequency), float32 [n, 3].  The logit of a token that is in ``seen`` is divided
+    by the repetition penalty if it is not negative and multiplied by it if it is; one with a count c > 0 then loses
+    frequency * c + presence.  ``counts`` is read only where ``seen`` has the token.
+    Biases (all three or none): those of row i are ``bias_values[b]`` (float32) for the tokens ``bias_ids[b]`` (int32), b from
+    ``bias_start[i]`` (int32 [n + 1]) to ``bias_start[i + 1]``; those of one token add up, ids outside the vocabulary are passed over.
+    Masks (both or none): row i may only be a token whose bit is set in row ``mask_rows[i]`` (int32 [n]; outside the table: no
+    mask) of ``masks`` (int32 [m, ceil(vocab / 32)], bit t % 32 of word t / 32); every other token's logit becomes -inf."""
+    what = "adjust_logits"
+    _need(logits.dim() == 2 and logits.shape == out.shape and logits.stride(1) == 1 and out.stride(1) == 1, what,
+          "logits and out are [n, vocab] with adjacent columns")
+    n, vocab = logits.shape
+    _need(out.dtype is torch.float32, what, "out is float32")
+    _need(n < 2 or (logits.stride(0) >= vocab and out.stride(0) >= vocab), what, "rows overlap")
+    same = (logits.data_ptr() == out.data_ptr() and logits.dtype is out.dtype and (n < 2 or logits.stride(0) == out.stride(0)))
+    _need(same or not _overlap(logits, out), what, "out shares memory with logits without being logits")
+    words = -(-vocab // 32)
+    n_slots = n_bias = n_masks = 0
+    if slots is not None or penalties is not None or counts is not None or seen is not None:
+        _need(slots is not None and penalties is not None and counts is not None and seen is not None, what,
+              "penalties need slots, penalties, counts and seen")
+        n_slots, v = _history(what, counts, seen)
+        _need(v == vocab, what, "the history has another vocabulary")
+        _need(slots.shape == (n,) and _ints(slots), what, "slots is a contiguous int32 [n]")
+        _need(penalties.shape == (n, 3) and penalties.dtype is torch.float32 and penalties.is_contiguous(), what,
+              "penalties is a contiguous float32 [n, 3]")
+    if bias_start is not None or bias_ids is not None or bias_values is not None:
+        _need(bias_start is not None and bias_ids is not None and bias_values is not None, what,
+              "biases need bias_start, bias_ids and bias_values")
+        n_bias = bias_ids.shape[0]
+        _need(bias_start.shape == (n + 1,) and _ints(bias_start) and bias_ids.dim() == 1 and _ints(bias_ids), what,
+              "bias_start is a contiguous int32 [n + 1], bias_ids a contiguous int32 vector")
+        _need(bias_values.shape == (n_bias,) and bias_values.dtype is torch.float32 and bias_values.is_contiguous(), what,
+              "bias_values is a contiguous float32 vector like bias_ids")
+    if mask_rows is not None or masks is not None:
+        _need(mask_rows is not None and masks is not None, what, "masks need mask_rows and masks")
+        _need(mask_rows.shape == (n,) and _ints(mask_rows), what, "mask_rows is a contiguous int32 [n]")
+        _need(masks.dim() == 2 and masks.shape[1] == words and _ints(masks), what,
+              "masks is a contiguous int32 [m, ceil(vocab / 32)]")
+        n_masks = masks.shape[0]
+    _here(what, logits=logits, out=out, slots=slots, penalties=penalties, counts=counts, seen=seen, bias_start=bias_start,
+          bias_ids=bias_ids, bias_values=bias_values, mask_rows=mask_rows, masks=masks)
+    _check(core().ie_adjust_logits(logits.data_ptr(), dtype_code(logits.dtype), out.data_ptr(), _ptr(slots), _ptr(penalties),
+                                   _ptr(counts), _ptr(seen), _ptr(bias_start), _ptr(bias_ids), _ptr(bias_values), _ptr(mask_rows),
+                                   _ptr(masks), n, vocab, logits.stride(0), out.stride(0), n_slots, n_bias, n_masks,
+                                   1 if same else 0, _stream()), what)
+
+
 # ------------------------------------------------- tensor-core attention (bfloat16)
 MMA_HEAD_DIMS = (64, 128)
 _mma: dict[tuple, object] = {}
@@ -1641,6 +1774,113 @@ def gemm_tcgen05(a: torch.Tensor, w: torch.Tensor, c: torch.Tensor, epi: str = "
 
 # ------------------------------------------- prompt-portion attention on tcgen05 (head sizes 64 and 128)
 _fa5_lib = None
+
+
+# ------------------------------------------------------------- 8-bit floating point
+FP8 = torch.float8_e4m3fn
+FP8_GROUP = 128          # columns (of a weight: rows too) that share a scale
+IE_E4M3 = 2
+_fp8_lib = None
+
+
+def fp8_library():
+    global _fp8_lib
+    if _fp8_lib is None:
+        lib = load_library("fp8", ["fp8_quantize.cu", "gemm_fp8.cu"], dict(BUILD_DEFINES.get("fp8", {})))
+        P, I, L = c_void_p, c_int, c_longlong
+        lib.ie_fp8_quantize_rows.argtypes = [P, I, P, P, I, I, L, L, L, L, P]
+        lib.ie_fp8_quantize_blocks.argtypes = [P, I, P, P, I, I, L, L, P]
+        lib.ie_gemm_fp8.argtypes = [P, I, P, P, P, P, I, I, I, I, L, L, L, L, L, P, P]
+        lib.ie_gemm_fp8_scratch.argtypes = [I, I]
+        for name in ("ie_fp8_quantize_rows", "ie_fp8_quantize_blocks", "ie_gemm_fp8"):
+            getattr(lib, name).restype = c_int
+        lib.ie_gemm_fp8_scratch.restype = c_longlong
+        _fp8_lib = lib
+    return _fp8_lib
+
+
+def fp8_empty(rows: int, cols: int, device) -> torch.Tensor:
+    """Room for the codes of a [rows, cols] matrix: rows 16 bytes (or a multiple) apart, as the kernels take them."""
+    return torch.empty((rows, max(16, -(-cols // 16) * 16)), dtype=FP8, device=device)[:, :cols]
+
+
+def _codes(what: str, name: str, t: torch.Tensor) -> None:
+    _need(t.dim() == 2 and t.dtype is FP8, what, f"{name} is a float8_e4m3fn matrix")
+    _need((t.stride(1) == 1 or t.shape[1] < 2) and t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0, what,
+          f"rows of {name} are adjacent codes and start on 16 bytes")
+
+
+def _rows_in(what: str, name: str, t: torch.Tensor) -> None:
+    _need(t.dim() == 2 and t.dtype in _CODES, what, f"{name} is a float32 or bfloat16 matrix")
+    _need(t.stride(1) == 1 or t.shape[1] < 2, what, f"columns of {name} are adjacent")
+
+
+def fp8_quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """x (float32 or bfloat16 [n, k]) as 8-bit floating point with a scale for each row and 128 columns:
+    ``codes`` (float8_e4m3fn [n, k], rows a multiple of 16 bytes apart) times ``scales`` (float32 [n, ceil(k / 128)], any strides).
+    A scale is the least power of two that brings the group's largest finite number to at most 448 (1 for zeros); a code is
+    the nearest e4m3 number to x / scale, ties to even, NaN for a number that is not finite."""
+    what = "fp8_quantize_rows"
+    _rows_in(what, "x", x)
+    _codes(what, "codes", codes)
+    n, k = x.shape
+    _need(codes.shape == x.shape, what, "codes has another shape than x")
+    _need(scales.shape == (n, -(-k // FP8_GROUP)) and scales.dtype is torch.float32, what, "scales is float32 [n, ceil(k / 128)]")
+    _here(what, x=x, codes=codes, scales=scales)
+    _check(fp8_library().ie_fp8_quantize_rows(x.data_ptr(), _CODES[x.dtype], codes.data_ptr(), scales.data_ptr(), n, k, x.stride(0),
+                                              codes.stride(0), scales.stride(0), scales.stride(1), _stream()), what)
+
+
+def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """The same for a weight: a scale for each block of 128 rows x 128 columns, ``scales`` contiguous
+    [ceil(n / 128), ceil(k / 128)]."""
+    what = "fp8_quantize_blocks"
+    _rows_in(what, "w", w)
+    _codes(what, "codes", codes)
+    n, k = w.shape
+    _need(codes.shape == w.shape, what, "codes has another shape than w")
+    _need(scales.shape == (-(-n // FP8_GROUP), -(-k // FP8_GROUP)) and scales.dtype is torch.float32 and scales.is_contiguous(), what,
+          "scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
+    _here(what, w=w, codes=codes, scales=scales)
+    _check(fp8_library().ie_fp8_quantize_blocks(w.data_ptr(), _CODES[w.dtype], codes.data_ptr(), scales.data_ptr(), n, k, w.stride(0),
+                                                codes.stride(0), _stream()), what)
+
+
+def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, x_scales: torch.Tensor | None = None) -> None:
+    """out (float32 or bfloat16 [m, n]) = x w^T in 8-bit floating point.  ``w`` (codes, [n, k]) with ``w_scales`` (float32, contiguous,
+    [ceil(n / 128), ceil(k / 128)], any positive numbers); ``x`` codes with ``x_scales`` (float32 [m, ceil(k / 128)], any strides), or
+    float32 / bfloat16 rows, which are quantised as ``fp8_quantize_rows`` does.  Codes lie as ``fp8_empty`` lays them out.  Sums are
+    float32: inside a block of 128 columns on the tensor cores, over the scaled blocks in registers."""
+    what = "gemm_fp8"
+    _codes(what, "w", w)
+    n, k = w.shape
+    m = x.shape[0]
+    _need(x.dim() == 2 and x.shape[1] == k and out.shape == (m, n), what, "x is [m, k], w [n, k], out [m, n]")
+    _need(out.dtype in _CODES and (out.stride(1) == 1 or n < 2) and (m < 2 or out.stride(0) >= n), what,
+          "out is a float32 or bfloat16 matrix of adjacent columns")
+    kb = -(-k // FP8_GROUP)
+    _need(w_scales.shape == (-(-n // FP8_GROUP), kb) and w_scales.dtype is torch.float32 and w_scales.is_contiguous(), what,
+          "w_scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
+    _need(k > 0, what, "k is 0")
+    scratch = None
+    if x.dtype is FP8:
+        _codes(what, "x", x)
+        _need(x_scales is not None and x_scales.shape == (m, kb) and x_scales.dtype is torch.float32, what,
+              "codes of x come with x_scales, float32 [m, ceil(k / 128)]")
+        code, s_row, s_col = IE_E4M3, x_scales.stride(0), x_scales.stride(1)
+    else:
+        _rows_in(what, "x", x)
+        _need(x_scales is None, what, "x_scales go with codes of x")
+        code, s_row, s_col = _CODES[x.dtype], 0, 0
+    _here(what, x=x, w=w, w_scales=w_scales, out=out, x_scales=x_scales)
+    if m == 0 or n == 0:
+        return
+    lib = fp8_library()
+    if code != IE_E4M3:
+        scratch = torch.empty(lib.ie_gemm_fp8_scratch(m, k), dtype=torch.uint8, device=x.device)
+    _check(lib.ie_gemm_fp8(x.data_ptr(), code, _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), _CODES[out.dtype],
+                           m, n, k, x.stride(0), s_row, s_col, w.stride(0), out.stride(0), _ptr(scratch), _stream()), what)
+
 
 
 def attention_tcgen05_library():
