@@ -5,7 +5,10 @@
 //
 // inner and outer sums in float32, one rounding to the output's type.
 #include "common.cuh"
-#include <cuda_fp8.h>
+#include <cooperative_groups.h>
+#include <cuda.h>
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -21,43 +24,368 @@ struct Fp8Params {
   int M, N, K;
   long long ldx, sx_row, sx_col, ldw, ldy;
   int y_bf16;
+  int y_vec;       // rows of y start on 16 bytes
+  int split;       // blocks of a cluster that share a tile
+  int stages;
 };
 
-__device__ __forceinline__ float code_value(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+// ------------------------------------------------------------------- tiles on the tensor cores
+// 128 rows x BN columns a tile.  One stage of the ring is one block of 128 codes of K (a 128-byte swizzle row), so one scale of x
+// a row and one of w for 128 columns hold for all of it: four MMAs of 32 codes make the block's sum in tensor memory from
+// nothing, and eight warps add it, scaled, to the sums that they keep in registers, while the MMAs of the next block fill the
+// other half of tensor memory.
+constexpr int BM = 128;
+// Twelve warps: TMA, MMA, two that do nothing, eight that sum.  A thread is launched with 168 registers (three warps a quarter of
+// the SM); the first four warps hand some of theirs on: 4 * 56 + 8 * 224 = 12 * 168.
+// (Only the wide tile, whose sums alone take 128 registers, needs it.)
+constexpr int TILE_THREADS = 384;
+constexpr int REGS_LAUNCH = 168, REGS_FEW = 56, REGS_MANY = 224;
+static_assert(REGS_FEW + 2 * REGS_MANY <= 3 * REGS_LAUNCH, "a share beyond what the block was launched with is never given out");
+constexpr unsigned SPIN_LIMIT = 1u << 20;
+constexpr int OUT_STAGE = 32 * 128;    // bytes of a summing warp's output tile: 32 rows x 128 bytes
+
+__device__ int g_fp8_error = 0;
+
+__device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  for (unsigned i = 0; i < SPIN_LIMIT; ++i) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+// shared-memory descriptor: K-major rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t smem_desc(uint32_t byte_addr) {
+  return (uint64_t)((byte_addr & 0x3FFFF) >> 4) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D float32, A and B e4m3, both K-major, 128 x n
+__device__ __forceinline__ constexpr uint32_t instr_desc(int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// two float32 multiply-adds in one instruction: acc += c * f, each of the two rounded as a single one is
+__device__ __forceinline__ void fma2(unsigned long long& acc, uint32_t c0, uint32_t c1, unsigned long long f) {
+  asm("{\n.reg .b64 c;\nmov.b64 c, {%1, %2};\nfma.rn.f32x2 %0, c, %3, %0;\n}" : "+l"(acc) : "r"(c0), "r"(c1), "l"(f));
+}
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+  return (unsigned long long)__float_as_uint(a) | ((unsigned long long)__float_as_uint(b) << 32);
+}
+__device__ __forceinline__ float low(unsigned long long v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high(unsigned long long v) { return __uint_as_float((uint32_t)(v >> 32)); }
+
+// 16 bytes of a row of y from column n: whole where they lie inside the matrix and on 16 bytes, else number by number
+__device__ __forceinline__ void store16(const Fp8Params& p, int m, int n, uint4 v) {
+  const int per = p.y_bf16 ? 8 : 4;
+  unsigned char* dst = (unsigned char*)p.y + ((long long)m * p.ldy + n) * (p.y_bf16 ? 2 : 4);
+  if (p.y_vec && n + per <= p.N) {
+    *reinterpret_cast<uint4*>(dst) = v;
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (p.y_bf16) {
+      if (n + 2 * j < p.N) reinterpret_cast<unsigned short*>(dst)[2 * j] = (unsigned short)w[j];
+      if (n + 2 * j + 1 < p.N) reinterpret_cast<unsigned short*>(dst)[2 * j + 1] = (unsigned short)(w[j] >> 16);
+    } else if (n + j < p.N) {
+      reinterpret_cast<uint32_t*>(dst)[j] = w[j];
+    }
+  }
+}
+__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// tiles of 32 x 32 results, one block of 32 columns at a time through shared memory
-__global__ void __launch_bounds__(256) gemm_fp8_kernel(Fp8Params p) {
-  __shared__ float xs[32][33], ws[32][33];
+// SPLIT: a tile's blocks of K are dealt out to the blocks of a cluster, whose sums come together through each other's shared
+// memory, in the order of K; else a block walks over tiles.
+template <int BN, bool SPLIT>
+__global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                                        const __grid_constant__ CUtensorMap map_w, Fp8Params p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];     // full[8], empty[8], acc_full[2], acc_empty[2]
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int failed;
+  constexpr uint32_t X_BYTES = BM * GROUP, STAGE = (BM + BN) * GROUP;
+  constexpr int COLS = BN / 2;                                    // columns of a summing warp: of one block of w's scales
+
   pdl_trigger();
-  pdl_wait();
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, kb = (p.K + GROUP - 1) / GROUP;
-  const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 32, n = n0 + tx;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int b = 0; b < kb; ++b) {
-    float in[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = b * GROUP; k0 < min(p.K, (b + 1) * GROUP); k0 += 32) {
-      __syncthreads();
-      for (int i = ty; i < 32; i += 8) {
-        xs[i][tx] = (m0 + i < p.M && k0 + tx < p.K) ? code_value(p.x[(m0 + i) * p.ldx + k0 + tx]) : 0.f;
-        ws[i][tx] = (n0 + i < p.N && k0 + tx < p.K) ? code_value(p.w[(n0 + i) * p.ldw + k0 + tx]) : 0.f;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t ring = (saddr(smem_raw) + 1023u) & ~1023u;
+  unsigned char* ring_ptr = smem_raw + (ring - saddr(smem_raw));
+  const uint32_t full0 = saddr(&bars[0]), empty0 = saddr(&bars[8]), acc_full0 = saddr(&bars[16]), acc_empty0 = saddr(&bars[18]);
+  const int k_blocks = (p.K + GROUP - 1) / GROUP, m_tiles = (p.M + BM - 1) / BM, tiles = m_tiles * ((p.N + BN - 1) / BN);
+  const int rank = SPLIT ? (int)(blockIdx.x % p.split) : 0;
+  const int t0 = SPLIT ? (int)(blockIdx.x / p.split) : (int)blockIdx.x, t_step = SPLIT ? tiles : (int)gridDim.x;
+  const int kb0 = SPLIT ? k_blocks * rank / p.split : 0, kb1 = SPLIT ? k_blocks * (rank + 1) / p.split : k_blocks;
+
+  if (tid == 0) {
+    failed = 0;
+    for (int s = 0; s < p.stages; ++s) {
+      bar_init(full0 + 8 * s, 1);
+      bar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      bar_init(acc_full0 + 8 * b, 1);
+      bar_init(acc_empty0 + 8 * b, 8);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_slot)), "n"(2 * BN) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();                                          // the codes of x come from the kernel ahead
+
+  if (warp < 4) {
+    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
+    if (warp == 0) {
+      if (lane == 0) {
+        int s = 0;
+        uint32_t phase = 0;
+        for (int t = t0; t < tiles && !failed; t += t_step) {
+          const int m0 = (t % m_tiles) * BM, n0 = (t / m_tiles) * BN;     // blocks side by side share a tile of the weight
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (failed || !bar_wait(empty0 + 8 * s, phase ^ 1)) { atomicExch(&g_fp8_error, 1); failed = 1; break; }
+            bar_expect(full0 + 8 * s, STAGE);
+            tma_load(ring + s * STAGE, &map_x, kb * GROUP, m0, full0 + 8 * s);
+            tma_load(ring + s * STAGE + X_BYTES, &map_w, kb * GROUP, n0, full0 + 8 * s);
+            if (++s == p.stages) { s = 0; phase ^= 1; }
+          }
+        }
+        if (failed) for (int i = 0; i < 2048; ++i) __nanosleep(64);      // copies under way still land in this block's memory
       }
-      __syncthreads();
-      for (int k = 0; k < 32; ++k)
-        for (int i = 0; i < 4; ++i) in[i] += xs[ty + 8 * i][k] * ws[tx][k];
+    } else if (warp == 1) {
+      if (lane == 0) {
+        int s = 0, it = 0;
+        uint32_t phase = 0;
+        for (int t = t0; t < tiles && !failed; t += t_step) {
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int buf = it & 1;
+            if (failed || !bar_wait(acc_empty0 + 8 * buf, ((uint32_t)(it >> 1) & 1u) ^ 1u)) { atomicExch(&g_fp8_error, 2); failed = 1; break; }
+            if (!bar_wait(full0 + 8 * s, phase)) { atomicExch(&g_fp8_error, 3); failed = 1; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t a = ring + s * STAGE, b = a + X_BYTES;
+#pragma unroll
+            for (int k = 0; k < GROUP / 32; ++k)
+              mma_fp8(tmem + (uint32_t)(buf * BN), smem_desc(a + 32 * k), smem_desc(b + 32 * k), instr_desc(BN), k > 0 ? 1u : 0u);
+            mma_commit(empty0 + 8 * s);                  // the stage has been read
+            mma_commit(acc_full0 + 8 * buf);             // the block's sum is there
+            if (++s == p.stages) { s = 0; phase ^= 1; }
+          }
+        }
+      }
     }
-    for (int i = 0; i < 4; ++i) {
-      const int m = m0 + ty + 8 * i;
-      if (m < p.M && n < p.N) acc[i] += p.sx[m * p.sx_row + b * p.sx_col] * p.sw[(long long)(n / GROUP) * kb + b] * in[i];
+  } else {
+    if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
+    const int quarter = warp & 3, half = (warp - 4) >> 2;          // tensor memory lanes 32 quarter .., columns COLS half ..
+    int it = 0;
+    bool ok = true;
+    for (int t = t0; t < tiles && ok; t += t_step) {
+      const int m0 = (t % m_tiles) * BM + quarter * 32, n0 = (t / m_tiles) * BN + half * COLS;
+      const float* sx = p.sx + min(m0 + lane, p.M - 1) * p.sx_row;
+      const float* sw = p.sw + (long long)min(n0 / GROUP, (p.N - 1) / GROUP) * k_blocks;
+      unsigned long long acc[COLS / 2];
+#pragma unroll
+      for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
+      float next = sx[kb0 * p.sx_col] * sw[kb0];
+#pragma unroll 1
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int buf = it & 1;
+        const unsigned long long f = pair(next, next);
+        if (kb + 1 < kb1) next = sx[(kb + 1) * p.sx_col] * sw[kb + 1];
+        ok = !failed && bar_wait(acc_full0 + 8 * buf, (uint32_t)(it >> 1) & 1u);
+        if (!ok) { atomicExch(&g_fp8_error, 4); failed = 1; }
+        ok = __all_sync(0xffffffffu, ok) && !failed;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < COLS / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + half * COLS + 32 * c), r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) fma2(acc[16 * c + j], r[2 * j], r[2 * j + 1], f);
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(acc_empty0 + 8 * buf);
+      }
+      if (!ok) break;
+      if (SPLIT) {
+        // the ring is free: every copy has landed and every MMA that read it has finished
+        float* row = reinterpret_cast<float*>(ring_ptr) + (quarter * 32 + lane) * (BN + 4) + half * COLS;
+#pragma unroll
+        for (int j = 0; j < COLS / 4; ++j)
+          *reinterpret_cast<float4*>(row + 4 * j) = make_float4(low(acc[2 * j]), high(acc[2 * j]), low(acc[2 * j + 1]), high(acc[2 * j + 1]));
+      } else {
+        // a lane holds a row: 128 bytes of each of the warp's 32 rows go through shared memory and out as whole lines (16-byte units
+        // swizzled by row, so that neither side has bank conflicts)
+        unsigned char* stage = ring_ptr + (size_t)p.stages * STAGE + (warp - 4) * OUT_STAGE;
+        const int per = p.y_bf16 ? 64 : 32, sw8 = lane & 7;
+#pragma unroll
+        for (int c = 0; c < COLS / 32; ++c) {
+          if (p.y_bf16) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              uint4 v;
+              v.x = two_bf16(low(acc[16 * c + 4 * u]), high(acc[16 * c + 4 * u]));
+              v.y = two_bf16(low(acc[16 * c + 4 * u + 1]), high(acc[16 * c + 4 * u + 1]));
+              v.z = two_bf16(low(acc[16 * c + 4 * u + 2]), high(acc[16 * c + 4 * u + 2]));
+              v.w = two_bf16(low(acc[16 * c + 4 * u + 3]), high(acc[16 * c + 4 * u + 3]));
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * (c & 1) + u) ^ sw8) << 4)) = v;
+            }
+            if ((c & 1) == 0) continue;
+          } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ sw8) << 4)) =
+                  make_uint4((uint32_t)acc[16 * c + 2 * u], (uint32_t)(acc[16 * c + 2 * u] >> 32), (uint32_t)acc[16 * c + 2 * u + 1],
+                             (uint32_t)(acc[16 * c + 2 * u + 1] >> 32));
+          }
+          __syncwarp();
+          const int first = n0 + 32 * c + 32 - per, u = lane & 7;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3), m = m0 + r, n = first + u * (per >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+            if (m < p.M && n < p.N) store16(p, m, n, v);
+          }
+          __syncwarp();
+        }
+      }
     }
   }
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty + 8 * i;
-    if (m >= p.M || n >= p.N) continue;
-    if (p.y_bf16) ((bf16*)p.y)[m * p.ldy + n] = __float2bfloat16_rn(acc[i]);
-    else ((float*)p.y)[m * p.ldy + n] = acc[i];
+
+  if (SPLIT) {
+    // every block of the cluster comes here, one whose waits ran out too
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int rows = BM / p.split, m0 = (t0 % m_tiles) * BM + rank * rows, n0 = (t0 / m_tiles) * BN;
+    const int per = p.y_bf16 ? 8 : 4, units = BN / per;
+    for (int i = tid; i < rows * units; i += TILE_THREADS) {
+      const int r = i / units, c = (i - r * units) * per, m = m0 + r;
+      if (m >= p.M || n0 + c >= p.N) continue;
+      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int q = 0; q < p.split; ++q) {
+        const float* from = reinterpret_cast<const float*>(cluster.map_shared_rank(ring_ptr, q)) + (rank * rows + r) * (BN + 4) + c;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          if (j >= per) break;
+          const float4 v = *reinterpret_cast<const float4*>(from + j);
+          sum[j] += v.x; sum[j + 1] += v.y; sum[j + 2] += v.z; sum[j + 3] += v.w;
+        }
+      }
+      uint4 v;
+      if (p.y_bf16) v = make_uint4(two_bf16(sum[0], sum[1]), two_bf16(sum[2], sum[3]), two_bf16(sum[4], sum[5]), two_bf16(sum[6], sum[7]));
+      else v = make_uint4(__float_as_uint(sum[0]), __float_as_uint(sum[1]), __float_as_uint(sum[2]), __float_as_uint(sum[3]));
+      store16(p, m, n0 + c, v);
+    }
+    cluster.sync();                                    // a block's memory is read until here
   }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * BN) : "memory");
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static std::atomic<EncodeTiledFn> known{nullptr};
+  EncodeTiledFn fn = known.load(std::memory_order_acquire);
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
+        qres == cudaDriverEntryPointSuccess)
+      known.store(fn = (EncodeTiledFn)ptr, std::memory_order_release);
+  }
+  return fn;
+}
+
+// codes [rows, cols], row pitch ld bytes: boxes of box_rows x 128 columns, zeros beyond the last column and row
+int make_map(CUtensorMap* map, const void* base, int rows, int cols, long long ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return IE_BAD_SIZE;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {(cuuint32_t)GROUP, (cuuint32_t)box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? IE_OK : IE_BAD_ALIGN;
+}
+
+template <int BN, bool SPLIT>
+int launch_tiles(Fp8Params p, int sms, cudaStream_t stream) {
+  CUtensorMap mx, mw;
+  int rc = make_map(&mx, p.x, p.M, p.K, p.ldx, BM);
+  if (rc) return rc;
+  rc = make_map(&mw, p.w, p.N, p.K, p.ldw, BN);
+  if (rc) return rc;
+  constexpr int STAGE = (BM + BN) * GROUP, STAGES = BN == 256 ? 4 : 6;
+  constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 8 * OUT_STAGE;
+  static_assert(SMEM <= 232448 - 1024, "shared memory of a block");
+  static_assert(!SPLIT || BM * (BN + 4) * 4 <= STAGES * STAGE, "the sums of a split tile fit the ring");
+  p.stages = STAGES;
+  static OncePerDevice once;
+  rc = once([] {
+    cudaFuncAttributes a;
+    const cudaError_t e = cudaFuncGetAttributes(&a, gemm_fp8_tile_kernel<BN, SPLIT>);
+    if (e != cudaSuccess) return (int)e;
+    if (BN == 256 && a.numRegs != REGS_LAUNCH) return IE_BAD_SIZE;      // built so that the shares do not add up
+    return (int)cudaFuncSetAttribute(gemm_fp8_tile_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+  });
+  if (rc) return rc;
+  const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  if (tiles * (SPLIT ? p.split : 1) > 0x7fffffffLL) return IE_BAD_SIZE;
+  if (SPLIT)
+    return launch_k_cluster(gemm_fp8_tile_kernel<BN, SPLIT>, p.split, (unsigned)(tiles * p.split), TILE_THREADS, SMEM, stream, mx, mw, p);
+  return launch_k(gemm_fp8_tile_kernel<BN, SPLIT>, (unsigned)(tiles < sms ? tiles : sms), TILE_THREADS, SMEM, stream, mx, mw, p);
 }
 
 }  // namespace
@@ -92,7 +420,22 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
   Fp8Params p;
   p.x = (const uint8_t*)x; p.sx = sx; p.w = (const uint8_t*)w; p.sw = sw; p.y = y; p.M = M; p.N = N; p.K = K;
   p.ldx = ldx; p.sx_row = sx_row; p.sx_col = sx_col; p.ldw = ldw; p.ldy = ldy; p.y_bf16 = y_dtype == IE_BF16;
-  const dim3 grid((N + 31) / 32, (M + 31) / 32);
-  if (grid.y > 65535) return IE_BAD_SIZE;
-  return launch_k(gemm_fp8_kernel, grid, 256, 0, stream, p);
+  p.y_vec = ((uintptr_t)y & 15) == 0 && ldy * (p.y_bf16 ? 2 : 4) % 16 == 0;
+  p.split = 1; p.stages = 0;
+  const int sms = device_sms();
+  if (sms <= 0) return IE_BAD_SIZE;
+  const long long wide = (long long)((M + BM - 1) / BM) * ((N + 255) / 256), tiles = (long long)((M + BM - 1) / BM) * ((N + 127) / 128);
+  if (wide >= sms) return launch_tiles<256, false>(p, sms, stream);
+  const int k_blocks = (K + GROUP - 1) / GROUP;
+  while (p.split < 8 && 2 * p.split * tiles <= sms && 4 * p.split <= k_blocks) p.split *= 2;
+  return p.split > 1 ? launch_tiles<128, true>(p, sms, stream) : launch_tiles<128, false>(p, sms, stream);
+}
+
+// reads and clears the word that a wait which ran out leaves (0: none)
+extern "C" int ie_gemm_fp8_error() {
+  int v = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_fp8_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v) cudaMemcpyToSymbol(g_fp8_error, &zero, sizeof(int));
+  return v;
 }

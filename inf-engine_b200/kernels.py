@@ -1795,8 +1795,14 @@ def fp8_library():
         for name in ("ie_fp8_quantize_rows", "ie_fp8_quantize_blocks", "ie_gemm_fp8"):
             getattr(lib, name).restype = c_int
         lib.ie_gemm_fp8_scratch.restype = c_longlong
+        lib.ie_gemm_fp8_error.restype = c_int
         _fp8_lib = lib
     return _fp8_lib
+
+
+def gemm_fp8_error() -> int:
+    """Reads and clears the error word that a timed-out wait of the 8-bit product leaves (0: none)."""
+    return int(fp8_library().ie_gemm_fp8_error())
 
 
 def fp8_empty(rows: int, cols: int, device) -> torch.Tensor:
@@ -2058,6 +2064,8 @@ def check_device_errors() -> None:
         found.append(f"tcgen05 product: code {e}")
     if _fa5_lib is not None and (e := attention_tcgen05_error()):
         found.append(f"tcgen05 attention: code {e}")
+    if _fp8_lib is not None and (e := gemm_fp8_error()):
+        found.append(f"8-bit product: code {e}")
     if found:
         raise KernelError("a kernel gave up a bounded wait; its results are not valid (" + "; ".join(found) + ")")
     if checks_enabled():
