@@ -26,15 +26,13 @@ struct Fp8Params {
   int y_bf16;
   int y_vec;       // rows of y start on 16 bytes
   int split;       // blocks of a cluster that share a tile
-  int stages;
 };
 
 // ------------------------------------------------------------------- tiles on the tensor cores
-// 128 rows x BN columns a tile.  One stage of the ring is one block of 128 codes of K (a 128-byte swizzle row), so one scale of x
-// a row and one of w for 128 columns hold for all of it: four MMAs of 32 codes make the block's sum in tensor memory from
-// nothing, and eight warps add it, scaled, to the sums that they keep in registers, while the MMAs of the next block fill the
-// other half of tensor memory.
-constexpr int BM = 128;
+// One stage of the ring is one block of 128 codes of K (a 128-byte swizzle row), so one scale of x a row and one of w for 128
+// columns hold for all of it: four MMAs of 32 codes make the block's sum in tensor memory from nothing, and eight warps add it,
+// scaled, to the sums that they keep in registers, while the MMAs of the next block fill the other half of tensor memory.
+constexpr int X_BYTES = 128 * GROUP, STAGE = 2 * X_BYTES, STAGES = 5;     // a block of K of 128 rows of x and 128 rows of w
 // Twelve warps: TMA, MMA, two that do nothing, eight that sum.  A thread is launched with 168 registers (three warps a quarter of
 // the SM); the first four warps hand some of theirs on: 4 * 56 + 8 * 224 = 12 * 168.
 // (Only the wide tile, whose sums alone take 128 registers, needs it.)
@@ -42,6 +40,7 @@ constexpr int TILE_THREADS = 384;
 constexpr int REGS_LAUNCH = 168, REGS_FEW = 56, REGS_MANY = 224;
 static_assert(REGS_FEW + 2 * REGS_MANY <= 3 * REGS_LAUNCH, "a share beyond what the block was launched with is never given out");
 constexpr unsigned SPIN_LIMIT = 1u << 20;
+constexpr int AHEAD = 8;               // blocks of K that the scales are asked for ahead
 constexpr int OUT_STAGE = 32 * 128;    // bytes of a summing warp's output tile: 32 rows x 128 bytes
 
 __device__ int g_fp8_error = 0;
@@ -56,45 +55,83 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+// an arrival at a barrier of any block of the cluster (an address of map_shared)
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t map_shared(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// one lane of a converged warp.  The warps that issue copies and MMAs run their loops whole and elect a lane for the issue alone:
+// what all lanes compute alike stays in the uniform registers that those instructions take (with a loop run by lane 0, moving it
+// there cost the MMA warp 900 cycles a block of K, of which its four MMAs are 512).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is != 0;
+}
+// waits for a phase; false when the limit is reached or another thread of the block has given up
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const volatile int* failed) {
   for (unsigned i = 0; i < SPIN_LIMIT; ++i) {
     uint32_t ok;
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     if (ok) return true;
+    if (*failed) return false;
   }
   return false;
 }
+// PAIR: the bytes are counted at a barrier that may be the other block's
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+  if (PAIR)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 // shared-memory descriptor: K-major rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart
 __device__ __forceinline__ uint64_t smem_desc(uint32_t byte_addr) {
   return (uint64_t)((byte_addr & 0x3FFFF) >> 4) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// D float32, A and B e4m3, both K-major, 128 x n
-__device__ __forceinline__ constexpr uint32_t instr_desc(int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+// D float32, A and B e4m3, both K-major, m x n
+__device__ __forceinline__ constexpr uint32_t instr_desc(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  if (PAIR)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// an arrival at the barrier (PAIR: at that of both blocks) when the MMAs so far have finished
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// the registers are named, so that nothing that reads them moves ahead of the wait
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+}
 
 // two float32 multiply-adds in one instruction: acc += c * f, each of the two rounded as a single one is
 __device__ __forceinline__ void fma2(unsigned long long& acc, uint32_t c0, uint32_t c1, unsigned long long f) {
@@ -130,136 +167,185 @@ __device__ __forceinline__ uint32_t two_bf16(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// SPLIT: a tile's blocks of K are dealt out to the blocks of a cluster, whose sums come together through each other's shared
-// memory, in the order of K; else a block walks over tiles.
-template <int BN, bool SPLIT>
+// PAIR: two blocks of a cluster make 256 x 256 of the result with MMAs over both SMs: each brings its 128 rows of x and HALF of the
+// 256 rows of w, so a block of K is 32 KB an SM where a tile of 128 x 256 alone takes 48 KB (and at 512 cycles of MMAs asks more
+// of the L2 than an SM gets from it).  The first block issues the MMAs; each block sums its own 128 rows.
+// SPLIT: 128 x 128; a tile's blocks of K are dealt out to the blocks of a cluster, whose sums come together through each other's
+// shared memory, in the order of K.  Neither: 128 x 128, a block walks over tiles.
+template <bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                         const __grid_constant__ CUtensorMap map_w, Fp8Params p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];     // full[8], empty[8], acc_full[2], acc_empty[2]
+  __shared__ __align__(8) unsigned long long bars[2 * STAGES + 4];     // full, empty, acc_full[2], acc_empty[2]
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
-  constexpr uint32_t X_BYTES = BM * GROUP, STAGE = (BM + BN) * GROUP;
-  constexpr int COLS = BN / 2;                                    // columns of a summing warp: of one block of w's scales
+  constexpr int TM = PAIR ? 256 : 128, TN = PAIR ? 256 : 128;          // the tile
+  constexpr int COLS = TN / 2;                                         // columns of a summing warp: of one block of w's scales
 
   pdl_trigger();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t ring = (saddr(smem_raw) + 1023u) & ~1023u;
   unsigned char* ring_ptr = smem_raw + (ring - saddr(smem_raw));
-  const uint32_t full0 = saddr(&bars[0]), empty0 = saddr(&bars[8]), acc_full0 = saddr(&bars[16]), acc_empty0 = saddr(&bars[18]);
-  const int k_blocks = (p.K + GROUP - 1) / GROUP, m_tiles = (p.M + BM - 1) / BM, tiles = m_tiles * ((p.N + BN - 1) / BN);
-  const int rank = SPLIT ? (int)(blockIdx.x % p.split) : 0;
-  const int t0 = SPLIT ? (int)(blockIdx.x / p.split) : (int)blockIdx.x, t_step = SPLIT ? tiles : (int)gridDim.x;
+  const uint32_t full0 = saddr(&bars[0]), empty0 = saddr(&bars[STAGES]), acc_full0 = saddr(&bars[2 * STAGES]), acc_empty0 = acc_full0 + 16;
+  const int k_blocks = (p.K + GROUP - 1) / GROUP, m_tiles = (p.M + TM - 1) / TM, tiles = m_tiles * ((p.N + TN - 1) / TN);
+  const int per_tile = PAIR ? 2 : SPLIT ? p.split : 1;                 // blocks of a tile (a cluster), and which of them this is
+  const int rank = (int)(blockIdx.x % per_tile);
+  const int t0 = (int)(blockIdx.x / per_tile), t_step = SPLIT ? tiles : (int)(gridDim.x / per_tile);
   const int kb0 = SPLIT ? k_blocks * rank / p.split : 0, kb1 = SPLIT ? k_blocks * (rank + 1) / p.split : k_blocks;
+  const int part = PAIR ? rank * 128 : 0;                              // this block's rows of x and of w in the tile
 
   if (tid == 0) {
     failed = 0;
-    for (int s = 0; s < p.stages; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       bar_init(full0 + 8 * s, 1);
       bar_init(empty0 + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
       bar_init(acc_full0 + 8 * b, 1);
-      bar_init(acc_empty0 + 8 * b, 8);
+      bar_init(acc_empty0 + 8 * b, PAIR ? 16 : 8);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_slot)), "n"(2 * BN) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_slot)), "n"(2 * TN) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_slot)), "n"(2 * TN) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  if (PAIR) cg::this_cluster().sync();                                 // the other block's barriers and tensor memory are there
+  else __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
-  pdl_wait();                                          // the codes of x come from the kernel ahead
+  pdl_wait();                                                          // the codes of x come from the kernel ahead
 
   if (warp < 4) {
-    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
+    if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
     if (warp == 0) {
-      if (lane == 0) {
-        int s = 0;
-        uint32_t phase = 0;
-        for (int t = t0; t < tiles && !failed; t += t_step) {
-          const int m0 = (t % m_tiles) * BM, n0 = (t / m_tiles) * BN;     // blocks side by side share a tile of the weight
-          for (int kb = kb0; kb < kb1; ++kb) {
-            if (failed || !bar_wait(empty0 + 8 * s, phase ^ 1)) { atomicExch(&g_fp8_error, 1); failed = 1; break; }
-            bar_expect(full0 + 8 * s, STAGE);
-            tma_load(ring + s * STAGE, &map_x, kb * GROUP, m0, full0 + 8 * s);
-            tma_load(ring + s * STAGE + X_BYTES, &map_w, kb * GROUP, n0, full0 + 8 * s);
-            if (++s == p.stages) { s = 0; phase ^= 1; }
+      const uint32_t first_full = PAIR ? map_shared(full0, 0) : full0;
+      int s = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = t0; t < tiles && ok; t += t_step) {
+        const int m0 = (t % m_tiles) * TM + part, n0 = (t / m_tiles) * TN + part;        // tiles side by side share the weight
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = __all_sync(0xffffffffu, bar_wait(empty0 + 8 * s, phase ^ 1, &failed));
+          if (!ok) { atomicExch(&g_fp8_error, 1); failed = 1; break; }
+          if (elect_one()) {
+            if (rank == 0 || !PAIR) bar_expect(full0 + 8 * s, (PAIR ? 2 : 1) * STAGE);
+            tma_load<PAIR>(ring + s * STAGE, &map_x, kb * GROUP, m0, first_full + 8 * s);
+            tma_load<PAIR>(ring + s * STAGE + X_BYTES, &map_w, kb * GROUP, n0, first_full + 8 * s);
           }
+          __syncwarp();
+          if (++s == STAGES) { s = 0; phase ^= 1; }
         }
-        if (failed) for (int i = 0; i < 2048; ++i) __nanosleep(64);      // copies under way still land in this block's memory
       }
-    } else if (warp == 1) {
-      if (lane == 0) {
-        int s = 0, it = 0;
-        uint32_t phase = 0;
-        for (int t = t0; t < tiles && !failed; t += t_step) {
-          for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const int buf = it & 1;
-            if (failed || !bar_wait(acc_empty0 + 8 * buf, ((uint32_t)(it >> 1) & 1u) ^ 1u)) { atomicExch(&g_fp8_error, 2); failed = 1; break; }
-            if (!bar_wait(full0 + 8 * s, phase)) { atomicExch(&g_fp8_error, 3); failed = 1; break; }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t a = ring + s * STAGE, b = a + X_BYTES;
+      if (failed) for (int i = 0; i < 2048; ++i) __nanosleep(64);        // copies under way still land in this block's memory
+    } else if (warp == 1 && (rank == 0 || !PAIR)) {
+      int s = 0, buf = 0;
+      uint32_t phase = 0, acc_phase = 1;
+      bool ok = true;
+      for (int t = t0; t < tiles && ok; t += t_step) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = __all_sync(0xffffffffu, bar_wait(acc_empty0 + 8 * buf, acc_phase, &failed));
+          if (!ok) { atomicExch(&g_fp8_error, 2); failed = 1; break; }
+          ok = __all_sync(0xffffffffu, bar_wait(full0 + 8 * s, phase, &failed));
+          if (!ok) { atomicExch(&g_fp8_error, 3); failed = 1; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t a = smem_desc(ring + s * STAGE), b = smem_desc(ring + s * STAGE + X_BYTES);
+          if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < GROUP / 32; ++k)
-              mma_fp8(tmem + (uint32_t)(buf * BN), smem_desc(a + 32 * k), smem_desc(b + 32 * k), instr_desc(BN), k > 0 ? 1u : 0u);
-            mma_commit(empty0 + 8 * s);                  // the stage has been read
-            mma_commit(acc_full0 + 8 * buf);             // the block's sum is there
-            if (++s == p.stages) { s = 0; phase ^= 1; }
+            for (int k = 0; k < GROUP / 32; ++k)               // 32 codes on: 2 units of 16 bytes in the descriptor's address
+              mma_fp8<PAIR>(tmem + (uint32_t)(buf * TN), a + 2 * k, b + 2 * k, instr_desc(TM, TN), k > 0 ? 1u : 0u);
+            mma_commit<PAIR>(empty0 + 8 * s);                  // the stage has been read
+            mma_commit<PAIR>(acc_full0 + 8 * buf);             // the block's sum is there
           }
+          __syncwarp();
+          if (++s == STAGES) { s = 0; phase ^= 1; }
+          buf ^= 1;
+          acc_phase ^= buf == 0 ? 1u : 0u;
         }
       }
     }
   } else {
-    if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
+    if (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
     const int quarter = warp & 3, half = (warp - 4) >> 2;          // tensor memory lanes 32 quarter .., columns COLS half ..
+    const uint32_t my_tmem = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * COLS);
+    const uint32_t first_empty = PAIR ? map_shared(acc_empty0, 0) : acc_empty0;
+    // The scales of a block come AHEAD blocks early into a slot of each thread's own (a load of theirs takes as long as several
+    // blocks' MMAs), on into the next tile.
+    const uint32_t slots = ring + STAGES * STAGE + 8 * OUT_STAGE + (tid - 128) * 8;
+    int ahead_t = t0, ahead_kb = kb0, ahead_slot = 0;
+    const float *ahead_sx = nullptr, *ahead_sw = nullptr;
+    const auto ask = [&]() {
+      if (ahead_t < tiles) {
+        if (ahead_kb == kb0) {
+          const int m = (ahead_t % m_tiles) * TM + part + quarter * 32 + lane, n = (ahead_t / m_tiles) * TN + half * COLS;
+          ahead_sx = p.sx + min(m, p.M - 1) * p.sx_row + kb0 * p.sx_col;
+          ahead_sw = p.sw + (long long)(min(n, p.N - 1) / GROUP) * k_blocks + kb0;
+        }
+        const uint32_t dst = slots + ahead_slot * 256 * 8;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(ahead_sx) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4), "l"(ahead_sw) : "memory");
+        ahead_sx += p.sx_col;
+        ++ahead_sw;
+        if (++ahead_kb == kb1) { ahead_kb = kb0; ahead_t += t_step; }
+      }
+      ahead_slot = (ahead_slot + 1) % AHEAD;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int i = 0; i < AHEAD - 1; ++i) ask();
     int it = 0;
     bool ok = true;
     for (int t = t0; t < tiles && ok; t += t_step) {
-      const int m0 = (t % m_tiles) * BM + quarter * 32, n0 = (t / m_tiles) * BN + half * COLS;
-      const float* sx = p.sx + min(m0 + lane, p.M - 1) * p.sx_row;
-      const float* sw = p.sw + (long long)min(n0 / GROUP, (p.N - 1) / GROUP) * k_blocks;
+      const int m0 = (t % m_tiles) * TM + part + quarter * 32, n0 = (t / m_tiles) * TN + half * COLS;
       unsigned long long acc[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
-      float next = sx[kb0 * p.sx_col] * sw[kb0];
 #pragma unroll 1
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int buf = it & 1;
-        const unsigned long long f = pair(next, next);
-        if (kb + 1 < kb1) next = sx[(kb + 1) * p.sx_col] * sw[kb + 1];
-        ok = !failed && bar_wait(acc_full0 + 8 * buf, (uint32_t)(it >> 1) & 1u);
+        ask();
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        float fx, fw;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(fx), "=f"(fw) : "r"(slots + (it % AHEAD) * 256 * 8) : "memory");
+        const unsigned long long f = pair(fx * fw, fx * fw);
+        ok = bar_wait(acc_full0 + 8 * buf, (uint32_t)(it >> 1) & 1u, &failed);
         if (!ok) { atomicExch(&g_fp8_error, 4); failed = 1; }
-        ok = __all_sync(0xffffffffu, ok) && !failed;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // 16 columns are under way while the 16 before them are added
+        uint32_t r[2][16];
+        tmem_ld16(my_tmem + (uint32_t)(buf * TN), r[0]);
 #pragma unroll
-        for (int c = 0; c < COLS / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + half * COLS + 32 * c), r);
-          tmem_ld_wait();
+        for (int c = 0; c < COLS / 16; ++c) {
+          tmem_ld_wait(r[c & 1]);
+          if (c + 1 < COLS / 16) {
+            tmem_ld16(my_tmem + (uint32_t)(buf * TN + 16 * (c + 1)), r[(c + 1) & 1]);
+          } else {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // all of it is in registers
+            __syncwarp();
+            if (lane == 0) { if (PAIR) bar_arrive_cluster(first_empty + 8 * buf); else bar_arrive(acc_empty0 + 8 * buf); }
+          }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) fma2(acc[16 * c + j], r[2 * j], r[2 * j + 1], f);
+          for (int j = 0; j < 8; ++j) fma2(acc[8 * c + j], r[c & 1][2 * j], r[c & 1][2 * j + 1], f);
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) bar_arrive(acc_empty0 + 8 * buf);
       }
       if (!ok) break;
       if (SPLIT) {
         // the ring is free: every copy has landed and every MMA that read it has finished
-        float* row = reinterpret_cast<float*>(ring_ptr) + (quarter * 32 + lane) * (BN + 4) + half * COLS;
+        float* row = reinterpret_cast<float*>(ring_ptr) + (quarter * 32 + lane) * (TN + 4) + half * COLS;
 #pragma unroll
         for (int j = 0; j < COLS / 4; ++j)
           *reinterpret_cast<float4*>(row + 4 * j) = make_float4(low(acc[2 * j]), high(acc[2 * j]), low(acc[2 * j + 1]), high(acc[2 * j + 1]));
       } else {
         // a lane holds a row: 128 bytes of each of the warp's 32 rows go through shared memory and out as whole lines (16-byte units
         // swizzled by row, so that neither side has bank conflicts)
-        unsigned char* stage = ring_ptr + (size_t)p.stages * STAGE + (warp - 4) * OUT_STAGE;
+        unsigned char* stage = ring_ptr + STAGES * STAGE + (warp - 4) * OUT_STAGE;
         const int per = p.y_bf16 ? 64 : 32, sw8 = lane & 7;
 #pragma unroll
         for (int c = 0; c < COLS / 32; ++c) {
@@ -295,24 +381,31 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
     }
   }
 
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (SPLIT) {
     // every block of the cluster comes here, one whose waits ran out too
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    const int rows = BM / p.split, m0 = (t0 % m_tiles) * BM + rank * rows, n0 = (t0 / m_tiles) * BN;
-    const int per = p.y_bf16 ? 8 : 4, units = BN / per;
+    const int rows = 128 / p.split, m0 = (t0 % m_tiles) * TM + rank * rows, n0 = (t0 / m_tiles) * TN;
+    const int per = p.y_bf16 ? 8 : 4, units = TN / per;
     for (int i = tid; i < rows * units; i += TILE_THREADS) {
       const int r = i / units, c = (i - r * units) * per, m = m0 + r;
       if (m >= p.M || n0 + c >= p.N) continue;
-      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int q = 0; q < p.split; ++q) {
-        const float* from = reinterpret_cast<const float*>(cluster.map_shared_rank(ring_ptr, q)) + (rank * rows + r) * (BN + 4) + c;
+      float4 part4[8][2];                              // all under way at once: one after the other they are 8 trips to another SM
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          if (j >= per) break;
-          const float4 v = *reinterpret_cast<const float4*>(from + j);
-          sum[j] += v.x; sum[j + 1] += v.y; sum[j + 2] += v.z; sum[j + 3] += v.w;
+      for (int q = 0; q < 8; ++q) {
+        if (q < p.split) {
+          const float* from = reinterpret_cast<const float*>(cluster.map_shared_rank(ring_ptr, q)) + (rank * rows + r) * (TN + 4) + c;
+          part4[q][0] = *reinterpret_cast<const float4*>(from);
+          if (per == 8) part4[q][1] = *reinterpret_cast<const float4*>(from + 4);
         }
+      }
+      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (q >= p.split) break;
+        sum[0] += part4[q][0].x; sum[1] += part4[q][0].y; sum[2] += part4[q][0].z; sum[3] += part4[q][0].w;
+        if (per == 8) { sum[4] += part4[q][1].x; sum[5] += part4[q][1].y; sum[6] += part4[q][1].z; sum[7] += part4[q][1].w; }
       }
       uint4 v;
       if (p.y_bf16) v = make_uint4(two_bf16(sum[0], sum[1]), two_bf16(sum[2], sum[3]), two_bf16(sum[4], sum[5]), two_bf16(sum[6], sum[7]));
@@ -322,10 +415,12 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
     cluster.sync();                                    // a block's memory is read until here
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  if (PAIR) cg::this_cluster().sync();                 // the other block's MMAs read this one's memory, and its warps arrive here
+  else __syncthreads();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * BN) : "memory");
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * TN) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * TN) : "memory");
   }
 }
 
@@ -346,13 +441,13 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// codes [rows, cols], row pitch ld bytes: boxes of box_rows x 128 columns, zeros beyond the last column and row
-int make_map(CUtensorMap* map, const void* base, int rows, int cols, long long ld, int box_rows) {
+// codes [rows, cols], row pitch ld bytes: boxes of 128 rows x 128 columns, zeros beyond the last column and row
+int make_map(CUtensorMap* map, const void* base, int rows, int cols, long long ld) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return IE_BAD_SIZE;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld};
-  const cuuint32_t box[2] = {(cuuint32_t)GROUP, (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {(cuuint32_t)GROUP, 128};
   const cuuint32_t elem[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -360,32 +455,32 @@ int make_map(CUtensorMap* map, const void* base, int rows, int cols, long long l
   return r == CUDA_SUCCESS ? IE_OK : IE_BAD_ALIGN;
 }
 
-template <int BN, bool SPLIT>
+template <bool PAIR, bool SPLIT>
 int launch_tiles(Fp8Params p, int sms, cudaStream_t stream) {
   CUtensorMap mx, mw;
-  int rc = make_map(&mx, p.x, p.M, p.K, p.ldx, BM);
+  int rc = make_map(&mx, p.x, p.M, p.K, p.ldx);
   if (rc) return rc;
-  rc = make_map(&mw, p.w, p.N, p.K, p.ldw, BN);
+  rc = make_map(&mw, p.w, p.N, p.K, p.ldw);
   if (rc) return rc;
-  constexpr int STAGE = (BM + BN) * GROUP, STAGES = BN == 256 ? 4 : 6;
-  constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 8 * OUT_STAGE;
+  constexpr size_t SMEM = 1024 + STAGES * STAGE + 8 * OUT_STAGE + AHEAD * 256 * 8;
   static_assert(SMEM <= 232448 - 1024, "shared memory of a block");
-  static_assert(!SPLIT || BM * (BN + 4) * 4 <= STAGES * STAGE, "the sums of a split tile fit the ring");
-  p.stages = STAGES;
+  static_assert(128 * (128 + 4) * 4 <= STAGES * STAGE, "the sums of a split tile fit the ring");
   static OncePerDevice once;
   rc = once([] {
     cudaFuncAttributes a;
-    const cudaError_t e = cudaFuncGetAttributes(&a, gemm_fp8_tile_kernel<BN, SPLIT>);
+    const cudaError_t e = cudaFuncGetAttributes(&a, gemm_fp8_tile_kernel<PAIR, SPLIT>);
     if (e != cudaSuccess) return (int)e;
-    if (BN == 256 && a.numRegs != REGS_LAUNCH) return IE_BAD_SIZE;      // built so that the shares do not add up
-    return (int)cudaFuncSetAttribute(gemm_fp8_tile_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+    if (PAIR && a.numRegs != REGS_LAUNCH) return IE_BAD_SIZE;           // built so that the shares do not add up
+    return (int)cudaFuncSetAttribute(gemm_fp8_tile_kernel<PAIR, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
   });
   if (rc) return rc;
-  const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-  if (tiles * (SPLIT ? p.split : 1) > 0x7fffffffLL) return IE_BAD_SIZE;
-  if (SPLIT)
-    return launch_k_cluster(gemm_fp8_tile_kernel<BN, SPLIT>, p.split, (unsigned)(tiles * p.split), TILE_THREADS, SMEM, stream, mx, mw, p);
-  return launch_k(gemm_fp8_tile_kernel<BN, SPLIT>, (unsigned)(tiles < sms ? tiles : sms), TILE_THREADS, SMEM, stream, mx, mw, p);
+  const long long side = PAIR ? 256 : 128, tiles = ((p.M + side - 1) / side) * ((p.N + side - 1) / side);
+  const long long cluster = PAIR ? 2 : SPLIT ? p.split : 1, room = sms / cluster;
+  const long long blocks = cluster * (SPLIT || tiles < room ? tiles : room);
+  if (tiles * cluster > 0x7fffffffLL || room < 1) return IE_BAD_SIZE;
+  if (PAIR || SPLIT)
+    return launch_k_cluster(gemm_fp8_tile_kernel<PAIR, SPLIT>, (int)cluster, (unsigned)blocks, TILE_THREADS, SMEM, stream, mx, mw, p);
+  return launch_k(gemm_fp8_tile_kernel<PAIR, SPLIT>, (unsigned)blocks, TILE_THREADS, SMEM, stream, mx, mw, p);
 }
 
 }  // namespace
@@ -421,14 +516,14 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
   p.x = (const uint8_t*)x; p.sx = sx; p.w = (const uint8_t*)w; p.sw = sw; p.y = y; p.M = M; p.N = N; p.K = K;
   p.ldx = ldx; p.sx_row = sx_row; p.sx_col = sx_col; p.ldw = ldw; p.ldy = ldy; p.y_bf16 = y_dtype == IE_BF16;
   p.y_vec = ((uintptr_t)y & 15) == 0 && ldy * (p.y_bf16 ? 2 : 4) % 16 == 0;
-  p.split = 1; p.stages = 0;
+  p.split = 1;
   const int sms = device_sms();
   if (sms <= 0) return IE_BAD_SIZE;
-  const long long wide = (long long)((M + BM - 1) / BM) * ((N + 255) / 256), tiles = (long long)((M + BM - 1) / BM) * ((N + 127) / 128);
-  if (wide >= sms) return launch_tiles<256, false>(p, sms, stream);
+  const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
+  if (M > 128 && (long long)((M + 255) / 256) * ((N + 255) / 256) >= sms / 2) return launch_tiles<true, false>(p, sms, stream);
   const int k_blocks = (K + GROUP - 1) / GROUP;
   while (p.split < 8 && 2 * p.split * tiles <= sms && 4 * p.split <= k_blocks) p.split *= 2;
-  return p.split > 1 ? launch_tiles<128, true>(p, sms, stream) : launch_tiles<128, false>(p, sms, stream);
+  return p.split > 1 ? launch_tiles<false, true>(p, sms, stream) : launch_tiles<false, false>(p, sms, stream);
 }
 
 // reads and clears the word that a wait which ran out leaves (0: none)
