@@ -16,35 +16,69 @@
 namespace {
 
 constexpr int GROUP = 128;
-constexpr int QT = 256;
+constexpr int QT = 256, BT = 512;      // threads of a block: rows, weights
 
-// 8 numbers of a row from column `col` (zeros from `cols` on)
-template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int col, int cols, bool vec, float (&v)[8]) {
-  if (vec && col + 8 <= cols) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + col);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(w[j] << 16);
-        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      }
+// 8 numbers of a row as they lie in memory; zeros from column `cols` on
+template <typename T> struct Raw8;
+template <> struct Raw8<bf16> {
+  uint4 u;
+  __device__ __forceinline__ void load(const bf16* __restrict__ row, int col, int cols, bool vec) {
+    if (vec && col + 8 <= cols) {
+      u = *reinterpret_cast<const uint4*>(row + col);
     } else {
-      const float4 a = *reinterpret_cast<const float4*>(row + col), b = *reinterpret_cast<const float4*>(row + col + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    }
-  } else {
+      uint32_t h[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? to_f32(row[col + j]) : 0.f;
+      for (int j = 0; j < 8; ++j) h[j] = col + j < cols ? __bfloat16_as_ushort(row[col + j]) : 0;
+      u = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    }
   }
-}
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* __restrict__ row, int col, int cols, bool vec) {
+    if (vec && col + 8 <= cols) {
+      a = *reinterpret_cast<const float4*>(row + col);
+      b = *reinterpret_cast<const float4*>(row + col + 4);
+    } else {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? row[col + j] : 0.f;
+      a = make_float4(v[0], v[1], v[2], v[3]);
+      b = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-__device__ __forceinline__ float largest8(const float (&v)[8]) {
-  float m = 0.f;
+// The largest magnitude of 8 numbers on top of m.  A maximum passes a NaN over, so only an infinity shows; a group whose maximum
+// is one looks again, number by number.
+__device__ __forceinline__ float largest8(const Raw8<float>& r, float m) {
+  m = fmaxf(m, fmaxf(fmaxf(fabsf(r.a.x), fabsf(r.a.y)), fmaxf(fabsf(r.a.z), fabsf(r.a.w))));
+  return fmaxf(m, fmaxf(fmaxf(fabsf(r.b.x), fabsf(r.b.y)), fmaxf(fabsf(r.b.z), fabsf(r.b.w))));
+}
+__device__ __forceinline__ float largest8(const Raw8<bf16>& r, float m) {
+  const auto two = [](uint32_t u) { u &= 0x7fff7fffu; return *reinterpret_cast<const __nv_bfloat162*>(&u); };
+  const __nv_bfloat162 h = __hmax2(__hmax2(two(r.u.x), two(r.u.y)), __hmax2(two(r.u.z), two(r.u.w)));
+  return fmaxf(m, fmaxf(__low2float(h), __high2float(h)));
+}
+template <typename T> __device__ __forceinline__ float largest_finite8(const Raw8<T>& r, float m) {
+  float v[8];
+  r.get(v);
 #pragma unroll
   for (int j = 0; j < 8; ++j) m = fmaxf(m, finite(v[j]) ? fabsf(v[j]) : 0.f);
   return m;
@@ -61,16 +95,18 @@ __device__ __forceinline__ int scale_exponent(float largest) {
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// 8 codes of v / 2^e, the first in the lowest byte
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inverse) {
+// 8 codes of the numbers times `inverse`, the first in the lowest byte.  A NaN becomes one; an infinity would become 448, so where
+// the group has one (`infinite`) it is made a NaN first.
+template <typename T> __device__ __forceinline__ uint2 codes8(const Raw8<T>& r, float inverse, bool infinite) {
+  float v[8];
+  r.get(v);
+  if (infinite) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = finite(v[j]) ? v[j] : __uint_as_float(0x7fffffffu);
+  }
   uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float2 p;
-    p.x = finite(v[2 * j]) ? v[2 * j] * inverse : __uint_as_float(0x7fffffffu);
-    p.y = finite(v[2 * j + 1]) ? v[2 * j + 1] * inverse : __uint_as_float(0x7fffffffu);
-    w[j] = __nv_cvt_float2_to_fp8x2(p, __NV_SATFINITE, __NV_E4M3);
-  }
+  for (int j = 0; j < 4; ++j) w[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j] * inverse, v[2 * j + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
   return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
@@ -84,60 +120,83 @@ __device__ __forceinline__ void store8(uint8_t* __restrict__ row, int col, int c
   }
 }
 
-// 16 lanes a group, 8 numbers a lane
-template <typename T>
+// 8 lanes a group, 2 x 8 numbers a lane; U groups of each 8 lanes are under way at once
+template <typename T, int U>
 __global__ void __launch_bounds__(QT) quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes,
                                                            float* __restrict__ scales, int rows, int cols, long long ldx,
                                                            long long ldc, long long s_row, long long s_col, int vec) {
-  pdl_trigger();
+  // the product behind this kernel asks for its weights as soon as it starts: it starts when every block here is past the wait, so
+  // what wrote them (the block quantiser, perhaps) has finished by then
   pdl_wait();
-  const int per_row = (cols + GROUP - 1) / GROUP;
-  const long long groups = (long long)rows * per_row;
-  const int lane16 = threadIdx.x & 15;
-  for (long long g = (long long)blockIdx.x * (QT / 16) + (threadIdx.x >> 4); g < groups; g += (long long)gridDim.x * (QT / 16)) {
-    const long long row = g / per_row;
-    const int b = (int)(g - row * per_row), col = b * GROUP + lane16 * 8;
-    float v[8];
-    load8(x + row * ldx, col, cols, vec != 0, v);
-    float m = largest8(v);
-    const unsigned half = 0xffffu << (threadIdx.x & 16);
+  pdl_trigger();
+  const unsigned per_row = (cols + GROUP - 1) / GROUP, groups = (unsigned)rows * per_row;
+  const int lane8 = threadIdx.x & 7;
+  const unsigned eight = 0xffu << (threadIdx.x & 24);
+  const unsigned g0 = blockIdx.x * (QT / 8 * U) + (threadIdx.x >> 3);
+  Raw8<T> raw[U][2];
+  unsigned row[U], block[U];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(half, m, o));
+  for (int i = 0; i < U; ++i) {
+    const unsigned g = min(g0 + i * (QT / 8), groups - 1);          // groups behind the last one: the last again, and not stored
+    row[i] = g / per_row;
+    block[i] = g - row[i] * per_row;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) raw[i][h].load(x + row[i] * ldx, block[i] * GROUP + 64 * h + lane8 * 8, cols, vec != 0);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (g0 + i * (QT / 8) >= groups) break;                         // all 8 lanes of a group alike
+    float m = largest8(raw[i][1], largest8(raw[i][0], 0.f));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(eight, m, o));
+    const bool infinite = !finite(m);
+    if (infinite) {
+      m = largest_finite8(raw[i][1], largest_finite8(raw[i][0], 0.f));
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(eight, m, o));
+    }
     const int e = scale_exponent(m);
-    store8(codes + row * ldc, col, cols, codes8(v, exp2i(-e)));
-    if (lane16 == 0) scales[row * s_row + b * s_col] = exp2i(e);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      store8(codes + row[i] * ldc, block[i] * GROUP + 64 * h + lane8 * 8, cols, codes8(raw[i][h], exp2i(-e), infinite));
+    if (lane8 == 0) scales[row[i] * s_row + block[i] * s_col] = exp2i(e);
   }
 }
 
-// a block of 128 x 128 a thread block: 16 threads a row, 8 rows a thread, all held in registers between the largest and the codes
+// a block of 128 x 128 a thread block: 16 threads a row, 4 rows a thread, all held in registers between the largest and the codes.
+// No trigger ahead of its end: a product behind it may ask for these codes before its wait.
 template <typename T>
-__global__ void __launch_bounds__(QT) quantize_blocks_kernel(const T* __restrict__ w, uint8_t* __restrict__ codes,
+__global__ void __launch_bounds__(BT) quantize_blocks_kernel(const T* __restrict__ w, uint8_t* __restrict__ codes,
                                                              float* __restrict__ scales, int rows, int cols, long long ldw,
                                                              long long ldc, int vec) {
+  constexpr int PER = GROUP * 16 / BT;
   __shared__ float red[33];
-  pdl_trigger();
   pdl_wait();
   const int col = blockIdx.x * GROUP + (threadIdx.x & 15) * 8;
   const long long row0 = (long long)blockIdx.y * GROUP + (threadIdx.x >> 4);
-  float v[8][8], m = 0.f;
+  Raw8<T> raw[PER];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const long long row = row0 + 16 * i;
-    if (row < rows) {
-      load8(w + row * ldw, col, cols, vec != 0, v[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    }
+  for (int i = 0; i < PER; ++i) {
+    const long long row = row0 + BT / 16 * i;
+    if (row < rows) raw[i].load(w + row * ldw, col, cols, vec != 0);
+    else raw[i].zero();
   }
+  float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, largest8(v[i]));
-  const int e = scale_exponent(block_max(m, red));
-  const float inverse = exp2i(-e);
+  for (int i = 0; i < PER; ++i) m = largest8(raw[i], m);
+  m = block_max(m, red);
+  const bool infinite = !finite(m);
+  if (infinite) {
+    m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const long long row = row0 + 16 * i;
-    if (row < rows) store8(codes + row * ldc, col, cols, codes8(v[i], inverse));
+    for (int i = 0; i < PER; ++i) m = largest_finite8(raw[i], m);
+    m = block_max(m, red);
+  }
+  const int e = scale_exponent(m);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const long long row = row0 + BT / 16 * i;
+    if (row < rows) store8(codes + row * ldc, col, cols, codes8(raw[i], exp2i(-e), infinite));
   }
   if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = exp2i(e);
 }
@@ -158,14 +217,16 @@ extern "C" int ie_fp8_quantize_rows(const void* x, int dtype, void* codes, float
   if (((uintptr_t)codes & 15) || ldc % 16) return IE_BAD_ALIGN;
   const int sms = device_sms();
   if (sms <= 0) return IE_BAD_SIZE;
-  const long long groups = (long long)rows * ((cols + GROUP - 1) / GROUP), blocks = (groups + QT / 16 - 1) / (QT / 16);
-  const int grid = (int)(blocks < 8LL * sms ? blocks : 8LL * sms);
+  const long long groups = (long long)rows * ((cols + GROUP - 1) / GROUP);
+  if (groups > 0x7fffffffLL) return IE_BAD_SIZE;
   const int vec = reads_vectors(x, ldx, dtype);
-  if (dtype == IE_F32)
-    return launch_k(quantize_rows_kernel<float>, grid, QT, 0, stream, (const float*)x, (uint8_t*)codes, scales, rows, cols, ldx, ldc,
-                    s_row, s_col, vec);
-  return launch_k(quantize_rows_kernel<bf16>, grid, QT, 0, stream, (const bf16*)x, (uint8_t*)codes, scales, rows, cols, ldx, ldc,
-                  s_row, s_col, vec);
+  // few groups: one for each 8 lanes, over as many SMs as there are; many: two, so that a thread has four loads under way
+  const int u = groups >= 32LL * 8 * sms ? 2 : 1;
+  const int grid = (int)((groups + QT / 8 * u - 1) / (QT / 8 * u));
+#define IE_ROWS(T, U) launch_k(quantize_rows_kernel<T, U>, grid, QT, 0, stream, (const T*)x, (uint8_t*)codes, scales, rows, cols, ldx, ldc, s_row, s_col, vec)
+  if (dtype == IE_F32) return u == 2 ? IE_ROWS(float, 2) : IE_ROWS(float, 1);
+  return u == 2 ? IE_ROWS(bf16, 2) : IE_ROWS(bf16, 1);
+#undef IE_ROWS
 }
 
 // w [rows, cols] -> codes and scales [ceil(rows / 128), ceil(cols / 128)], contiguous
@@ -178,6 +239,6 @@ extern "C" int ie_fp8_quantize_blocks(const void* w, int dtype, void* codes, flo
   if (grid.y > 65535) return IE_BAD_SIZE;
   const int vec = reads_vectors(w, ldw, dtype);
   if (dtype == IE_F32)
-    return launch_k(quantize_blocks_kernel<float>, grid, QT, 0, stream, (const float*)w, (uint8_t*)codes, scales, rows, cols, ldw, ldc, vec);
-  return launch_k(quantize_blocks_kernel<bf16>, grid, QT, 0, stream, (const bf16*)w, (uint8_t*)codes, scales, rows, cols, ldw, ldc, vec);
+    return launch_k(quantize_blocks_kernel<float>, grid, BT, 0, stream, (const float*)w, (uint8_t*)codes, scales, rows, cols, ldw, ldc, vec);
+  return launch_k(quantize_blocks_kernel<bf16>, grid, BT, 0, stream, (const bf16*)w, (uint8_t*)codes, scales, rows, cols, ldw, ldc, vec);
 }
