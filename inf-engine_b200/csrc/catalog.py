@@ -10,7 +10,7 @@ def all_build_requests():
     reqs = [("core", LIBRARIES["core"], {}, [])]
     reqs.append(("stream", ["gemm_stream.cu", "gemm_stream_tma.cu"], {}, []))
     reqs.append(("tcgen05", ["gemm_tcgen05.cu"], {}, []))
-    reqs.append(("fp8", ["fp8_quantize.cu", "gemm_fp8.cu"], {}, []))
+    reqs.append(("fp8", ["fp8_quantize.cu", "gemm_fp8.cu"], {}, ["fp8_codes.cuh"]))
     reqs.append(("attn_tcgen05", ["attention_tcgen05.cu"], {}, []))
     reqs.append(("attn_tcgen05_exact", ["attention_tcgen05.cu"], {"IE_FA_EXACT": 1}, []))
     for hd in (64, 128):

@@ -4,7 +4,7 @@
 //   y[m, n] = sum_b sx[m, b] sw[n / 128, b]  sum_{k in block b} x[m, k] w[n, k]
 //
 // inner and outer sums in float32, one rounding to the output's type.
-#include "common.cuh"
+#include "fp8_codes.cuh"
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -12,7 +12,6 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int GROUP = 128;
 enum { IE_E4M3 = 2 };      // dtype code of an operand that is quantised already
 
 struct Fp8Params {
@@ -29,6 +28,9 @@ struct Fp8Params {
   // the kernel ahead is the quantiser of x, whose blocks are past their own wait when one of this kernel starts: whatever wrote the
   // weights has finished then, so they may be asked for before this kernel's wait
   int early;
+  // x in bfloat16 where the product quantises it itself; whether its rows can be read 16 bytes at a time
+  const void* raw;
+  int raw_vec;
 };
 
 // ------------------------------------------------------------------- tiles on the tensor cores
@@ -544,7 +546,7 @@ constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32;
 __device__ __forceinline__ uint4 codes_to_the_end(const uint8_t* row, int k, int K) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (k < K) {
-    v = __ldg(reinterpret_cast<const uint4*>(row + k));
+    v = *reinterpret_cast<const uint4*>(row + k);
     const int n = K - k;
     uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
@@ -567,8 +569,59 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NT, int R>
+// The same 16 x 2 numbers of a row of x in bfloat16, and their codes.  A group's 128 columns lie with the four lanes of a row, so its
+// largest number is two exchanges away, and quantising here (as fp8_quantize.cu does) saves a kernel where the weight has few rows.
+struct RawRow { uint4 u[2][2]; };
+__device__ __forceinline__ RawRow raw_row(const bf16* row, int k, int K, bool whole) {
+  RawRow r;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = k + 64 * c + 8 * h;
+      if (whole) {
+        r.u[c][h] = *reinterpret_cast<const uint4*>(row + at);
+      } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = at + j < K ? __bfloat16_as_ushort(row[at + j]) : 0;
+        r.u[c][h] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+      }
+    }
+  return r;
+}
+__device__ __forceinline__ void quantize_row(const RawRow& r, uint4 (&codes)[2], float& scale) {
+  float m = 0.f;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) m = largest8(Raw8<bf16>{r.u[c][h]}, m);
+#pragma unroll
+  for (int o = 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const bool infinite = !finite(m);
+  if (__any_sync(0xffffffffu, infinite)) {
+    float f = 0.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f = largest_finite8(Raw8<bf16>{r.u[c][h]}, f);
+#pragma unroll
+    for (int o = 2; o > 0; o >>= 1) f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, o));
+    m = f;
+  }
+  const int e = scale_exponent(m);
+  scale = exp2i(e);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const uint2 a = codes8(Raw8<bf16>{r.u[c][0]}, exp2i(-e), infinite), b = codes8(Raw8<bf16>{r.u[c][1]}, exp2i(-e), infinite);
+    codes[c] = make_uint4(a.x, a.y, b.x, b.y);
+  }
+}
+
+// RAW: x comes in bfloat16 and is quantised here (one tile of 8 rows)
+template <int NT, int R, bool RAW>
 __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params p, int ks) {
+  static_assert(!RAW || NT == 1, "registers for one tile of raw rows");
   __shared__ float sums[FEW_WARPS][16 * R][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int groups = FEW_WARPS / ks, slice = warp % ks, k_blocks = (p.K + GROUP - 1) / GROUP;
@@ -599,31 +652,40 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params 
   const uint8_t* x_row = p.x + min(g, p.M - 1) * p.ldx + 16 * t;
   const uint8_t* x_row8 = NT == 1 ? nullptr : p.x + min(8 + g, p.M - 1) * p.ldx + 16 * t;
   const float* sx = p.sx + min(2 * t, p.M - 1) * p.sx_row;                        // rows of x beyond the last make results that nobody reads
-  uint4 xs[2][NT][2];
+  uint4 xs[2][RAW ? 1 : NT][2];
   float fs[2][2 * NT + 1];
+  RawRow raw[2];
+  const bf16* raw_at = (const bf16*)p.raw + min(g, p.M - 1) * p.ldx;
+  const auto ask_raw = [&](RawRow& to, float& f, int kb) {
+    f = sw[kb];
+    to = raw_row(raw_at, kb * GROUP + 16 * t, p.K, p.raw_vec && (kb + 1) * GROUP <= p.K);
+  };
   const auto ask_x = [&](uint4 (&to)[NT][2], float (&f)[2 * NT + 1], int kb) {
     const int k = kb * GROUP;
-    f[2 * NT] = __ldg(sw + kb);
+    f[2 * NT] = sw[kb];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const uint8_t* row = i == 0 ? x_row : x_row8;
       if (k + GROUP <= p.K) {
-        to[i][0] = __ldg(reinterpret_cast<const uint4*>(row + k));
-        to[i][1] = __ldg(reinterpret_cast<const uint4*>(row + k + 64));
+        to[i][0] = *reinterpret_cast<const uint4*>(row + k);
+        to[i][1] = *reinterpret_cast<const uint4*>(row + k + 64);
       } else {
         to[i][0] = codes_to_the_end(row - 16 * t, k + 16 * t, p.K);
         to[i][1] = codes_to_the_end(row - 16 * t, k + 16 * t + 64, p.K);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        f[2 * i + j] = __ldg(sx + (min(8 * i + 2 * t + j, p.M - 1) - min(2 * t, p.M - 1)) * p.sx_row + kb * p.sx_col);
+        f[2 * i + j] = sx[(min(8 * i + 2 * t + j, p.M - 1) - min(2 * t, p.M - 1)) * p.sx_row + kb * p.sx_col];
     }
   };
   pdl_trigger();
   if (p.early && kb0 < kb1) ask(w[0], kb0);
   pdl_wait();
   if (!p.early && kb0 < kb1) ask(w[0], kb0);
-  if (kb0 < kb1) ask_x(xs[0], fs[0], kb0);
+  if (kb0 < kb1) {
+    if constexpr (RAW) ask_raw(raw[0], fs[0][2 * NT], kb0);
+    else ask_x(xs[0], fs[0], kb0);
+  }
   float acc[R][NT][4];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -664,12 +726,32 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params 
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[r][i][j] = fmaf(in[r][i][j], f[2 * i + (j & 1)] * f[2 * NT], acc[r][i][j]);
   };
-  for (int kb = kb0; kb < kb1; kb += 2) {
-    if (kb + 1 < kb1) { ask(w[1], kb + 1); ask_x(xs[1], fs[1], kb + 1); }
-    add(w[0], xs[0], fs[0]);
-    if (kb + 1 < kb1) {
-      if (kb + 2 < kb1) { ask(w[0], kb + 2); ask_x(xs[0], fs[0], kb + 2); }
-      add(w[1], xs[1], fs[1]);
+  if constexpr (RAW) {
+    const auto add_raw = [&](const uint4 (&from)[2 * R][2], const RawRow& r, float fw) {
+      uint4 x[1][2];
+      float f[3], scale;
+      quantize_row(r, x[0], scale);
+      f[0] = __shfl_sync(0xffffffffu, scale, 8 * t);            // rows 2 t and 2 t + 1 of x are lanes 8 t .. and 8 t + 4 ..
+      f[1] = __shfl_sync(0xffffffffu, scale, 8 * t + 4);
+      f[2] = fw;
+      add(from, x, f);
+    };
+    for (int kb = kb0; kb < kb1; kb += 2) {
+      if (kb + 1 < kb1) { ask(w[1], kb + 1); ask_raw(raw[1], fs[1][2 * NT], kb + 1); }
+      add_raw(w[0], raw[0], fs[0][2 * NT]);
+      if (kb + 1 < kb1) {
+        if (kb + 2 < kb1) { ask(w[0], kb + 2); ask_raw(raw[0], fs[0][2 * NT], kb + 2); }
+        add_raw(w[1], raw[1], fs[1][2 * NT]);
+      }
+    }
+  } else {
+    for (int kb = kb0; kb < kb1; kb += 2) {
+      if (kb + 1 < kb1) { ask(w[1], kb + 1); ask_x(xs[1], fs[1], kb + 1); }
+      add(w[0], xs[0], fs[0]);
+      if (kb + 1 < kb1) {
+        if (kb + 2 < kb1) { ask(w[0], kb + 2); ask_x(xs[0], fs[0], kb + 2); }
+        add(w[1], xs[1], fs[1]);
+      }
     }
   }
 #pragma unroll
@@ -690,17 +772,20 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params 
   }
 }
 
-template <int NT, int R>
+template <int NT, int R, bool RAW>
 int launch_few_rows(const Fp8Params& p, int sms, cudaStream_t stream) {
   const int groups = (p.N + 16 * R - 1) / (16 * R), k_blocks = (p.K + GROUP - 1) / GROUP;
   int ks = 1;
   while (ks < 8 && (long long)groups * ks < 8LL * sms && 2 * ks <= k_blocks) ks *= 2;
   const int per = FEW_WARPS / ks, grid = (groups + per - 1) / per;
-  return launch_k(gemm_fp8_few_kernel<NT, R>, grid, FEW_THREADS, 0, stream, p, ks);
+  return launch_k(gemm_fp8_few_kernel<NT, R, RAW>, grid, FEW_THREADS, 0, stream, p, ks);
 }
+// whether the product of few rows in bfloat16 quantises them itself
+bool few_takes_raw(int M, int N, int sms) { return M <= 8 && N < 32 * sms; }
 int launch_few(const Fp8Params& p, int sms, cudaStream_t stream) {
-  if (p.M > 8) return launch_few_rows<2, 1>(p, sms, stream);
-  return p.N >= 32 * sms ? launch_few_rows<1, 2>(p, sms, stream) : launch_few_rows<1, 1>(p, sms, stream);
+  if (p.raw) return launch_few_rows<1, 1, true>(p, sms, stream);
+  if (p.M > 8) return launch_few_rows<2, 1, false>(p, sms, stream);
+  return p.N >= 32 * sms ? launch_few_rows<1, 2, false>(p, sms, stream) : launch_few_rows<1, 1, false>(p, sms, stream);
 }
 
 }  // namespace
@@ -710,8 +795,8 @@ extern "C" int ie_fp8_quantize_rows(const void* x, int dtype, void* codes, float
                                     long long ldc, long long s_row, long long s_col, cudaStream_t stream);
 
 // bytes of scratch that the product of unquantised rows takes: their codes, then their scales [K / 128][M]
-extern "C" long long ie_gemm_fp8_scratch(int M, int K) {
-  if (M <= 0 || K <= 0) return 0;
+extern "C" long long ie_gemm_fp8_scratch(int x_dtype, int M, int N, int K) {
+  if (M <= 0 || K <= 0 || x_dtype == IE_E4M3 || (x_dtype == IE_BF16 && few_takes_raw(M, N, device_sms()))) return 0;
   return (long long)M * ((K + 15) / 16 * 16) + 4LL * M * ((K + GROUP - 1) / GROUP);
 }
 
@@ -723,6 +808,19 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
   if (K <= 0) return IE_BAD_SIZE;
   if (y_dtype != IE_F32 && y_dtype != IE_BF16) return IE_BAD_DTYPE;
   if (((uintptr_t)w & 15) || ldw % 16) return IE_BAD_ALIGN;
+  const int sms = device_sms();
+  if (sms <= 0) return IE_BAD_SIZE;
+  Fp8Params p;
+  p.w = (const uint8_t*)w; p.sw = sw; p.y = y; p.M = M; p.N = N; p.K = K; p.ldw = ldw; p.ldy = ldy; p.y_bf16 = y_dtype == IE_BF16;
+  p.y_vec = ((uintptr_t)y & 15) == 0 && ldy * (p.y_bf16 ? 2 : 4) % 16 == 0;
+  p.split = 1;
+  p.early = 0;
+  p.raw = nullptr;
+  if (x_dtype == IE_BF16 && few_takes_raw(M, N, sms)) {
+    p.raw = x; p.raw_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
+    p.x = nullptr; p.sx = nullptr; p.ldx = ldx; p.sx_row = p.sx_col = 0;
+    return launch_few(p, sms, stream);
+  }
   if (x_dtype != IE_E4M3) {
     if (scratch == nullptr || ((uintptr_t)scratch & 15)) return IE_BAD_ALIGN;
     const long long pitch = (K + 15) / 16 * 16;
@@ -730,16 +828,10 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
     const int rc = ie_fp8_quantize_rows(x, x_dtype, scratch, scales, M, K, ldx, pitch, 1, M, stream);
     if (rc) return rc;
     x = scratch; ldx = pitch; sx = scales; sx_row = 1; sx_col = M;
+    p.early = 1;
   }
   if (((uintptr_t)x & 15) || ldx % 16) return IE_BAD_ALIGN;
-  Fp8Params p;
-  p.x = (const uint8_t*)x; p.sx = sx; p.w = (const uint8_t*)w; p.sw = sw; p.y = y; p.M = M; p.N = N; p.K = K;
-  p.ldx = ldx; p.sx_row = sx_row; p.sx_col = sx_col; p.ldw = ldw; p.ldy = ldy; p.y_bf16 = y_dtype == IE_BF16;
-  p.y_vec = ((uintptr_t)y & 15) == 0 && ldy * (p.y_bf16 ? 2 : 4) % 16 == 0;
-  p.split = 1;
-  p.early = x_dtype != IE_E4M3;
-  const int sms = device_sms();
-  if (sms <= 0) return IE_BAD_SIZE;
+  p.x = (const uint8_t*)x; p.sx = sx; p.ldx = ldx; p.sx_row = sx_row; p.sx_col = sx_col;
   if (M <= 16) return launch_few(p, sms, stream);
   const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
   // More tiles of 128 x 128 than SMs: pairs take less per result (512 x 8192 x 2048, 256 tiles: 15.8 us against 20.8; at 200 x 2048 x

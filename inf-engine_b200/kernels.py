@@ -1087,31 +1087,33 @@ def sample(logits: torch.Tensor, rows: torch.Tensor, out: torch.Tensor) -> None:
 
 
 # ------------------------------------------- a request's history, and the logits that it changes
-def _need(holds: bool, what: str, why: str) -> None:
-    if not holds:
-        raise KernelError(f"{what}: refused ({why})")
+# Their kernels take two to three microseconds in a decode step, no longer than checking a dozen tensors takes if every check is a
+# call: conditions stand in line, and a refusal is made only where one fails.
+def _refuse(what: str, why: str) -> None:
+    raise KernelError(f"{what}: refused ({why})")
 
 
-def _here(what: str, **tensors: torch.Tensor | None) -> None:
-    """The tensors lie on the current device, whose stream the kernels go to."""
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if dev is None and t.is_cuda:
-            dev = torch._C._cuda_getDevice()
-        if not t.is_cuda or t.get_device() != dev:
-            raise KernelError(f"{what}: {name} is on {t.device}, kernels run on tensors of the current device")
+def _away(what: str, *tensors: torch.Tensor | None) -> None:
+    """Says which of the tensors are not on the current device, whose stream the kernels go to."""
+    where = ", ".join(sorted({str(t.device) for t in tensors if t is not None}))
+    raise KernelError(f"{what}: refused (tensors on {where}; kernels run on tensors of the current device)")
 
 
-def _ints(t: torch.Tensor) -> bool:
-    return t.dtype is torch.int32 and t.is_contiguous()
+def _here(t: torch.Tensor) -> int:
+    """The index of the current device if ``t`` lies on it, else -2 (no tensor's)."""
+    d = t.get_device()
+    return d if d >= 0 and d == torch._C._cuda_getDevice() else -2
+
+
+_I32, _F32 = torch.int32, torch.float32
 
 
 def _history(what: str, counts: torch.Tensor, seen: torch.Tensor) -> tuple[int, int]:
-    _need(counts.dim() == 2 and _ints(counts), what, "counts is a contiguous int32 [slots, vocab]")
+    if counts.dim() != 2 or counts.dtype is not _I32 or not counts.is_contiguous():
+        _refuse(what, "counts is a contiguous int32 [slots, vocab]")
     n_slots, vocab = counts.shape
-    _need(seen.shape == (n_slots, -(-vocab // 32)) and _ints(seen), what, "seen is a contiguous int32 [slots, ceil(vocab / 32)]")
+    if seen.shape != (n_slots, (vocab + 31) // 32) or seen.dtype is not _I32 or not seen.is_contiguous():
+        _refuse(what, "seen is a contiguous int32 [slots, ceil(vocab / 32)]")
     return n_slots, vocab
 
 
@@ -1120,8 +1122,10 @@ def history_reset(counts: torch.Tensor, seen: torch.Tensor, slots: torch.Tensor)
     negative, or beyond the table, is passed over.  ``counts`` int32 [slots, vocab]; ``seen`` int32 [slots, ceil(vocab / 32)],
     bit t % 32 of word t / 32."""
     n_slots, vocab = _history("history_reset", counts, seen)
-    _need(slots.dim() == 1 and _ints(slots), "history_reset", "slots is a contiguous int32 [n]")
-    _here("history_reset", counts=counts, seen=seen, slots=slots)
+    if slots.dim() != 1 or slots.dtype is not _I32 or not slots.is_contiguous():
+        _refuse("history_reset", "slots is a contiguous int32 [n]")
+    if not _here(counts) == seen.get_device() == slots.get_device():
+        _away("history_reset", counts, seen, slots)
     _check(core().ie_history_reset(counts.data_ptr(), seen.data_ptr(), slots.data_ptr(), slots.shape[0], n_slots, vocab, _stream()),
            "history_reset")
 
@@ -1132,16 +1136,33 @@ def history_append(counts: torch.Tensor, seen: torch.Tensor, tokens: torch.Tenso
     ascending; None: one token a slot) belong to slot r, and the first ``n_prompt[r]`` of them (int32 [R]; None: none) to its prompt:
     those set the bit in ``seen``; every other token also adds one to ``counts``.  A token outside the vocabulary, or of a slot that
     is negative or beyond the table, is passed over.  Tokens and slots may come more than once."""
-    n_slots, vocab = _history("history_append", counts, seen)
+    what = "history_append"
+    n_slots, vocab = _history(what, counts, seen)
+    if (tokens.dim() != 1 or tokens.dtype is not _I32 or not tokens.is_contiguous() or slots.dim() != 1 or slots.dtype is not _I32
+            or not slots.is_contiguous()):
+        _refuse(what, "tokens and slots are contiguous int32 vectors")
     n, r = tokens.shape[0], slots.shape[0]
-    _need(tokens.dim() == 1 and _ints(tokens) and slots.dim() == 1 and _ints(slots), "history_append",
-          "tokens and slots are contiguous int32 vectors")
-    _need(starts is not None or n == r, "history_append", "without starts there is one token a slot")
-    _need(starts is None or (starts.shape == (r + 1,) and _ints(starts)), "history_append", "starts is a contiguous int32 [slots + 1]")
-    _need(n_prompt is None or (n_prompt.shape == (r,) and _ints(n_prompt)), "history_append", "n_prompt is a contiguous int32 [slots]")
-    _here("history_append", counts=counts, seen=seen, tokens=tokens, slots=slots, starts=starts, n_prompt=n_prompt)
-    _check(core().ie_history_append(counts.data_ptr(), seen.data_ptr(), tokens.data_ptr(), slots.data_ptr(), _ptr(starts),
-                                    _ptr(n_prompt), n, r, n_slots, vocab, _stream()), "history_append")
+    dev = _here(counts)
+    if not dev == seen.get_device() == tokens.get_device() == slots.get_device():
+        dev = -2
+    if starts is None:
+        if n != r:
+            _refuse(what, "without starts there is one token a slot")
+    else:
+        if starts.shape != (r + 1,) or starts.dtype is not _I32 or not starts.is_contiguous():
+            _refuse(what, "starts is a contiguous int32 [slots + 1]")
+        if starts.get_device() != dev:
+            dev = -2
+    if n_prompt is not None:
+        if n_prompt.shape != (r,) or n_prompt.dtype is not _I32 or not n_prompt.is_contiguous():
+            _refuse(what, "n_prompt is a contiguous int32 [slots]")
+        if n_prompt.get_device() != dev:
+            dev = -2
+    if dev < 0:
+        _away(what, counts, seen, tokens, slots, starts, n_prompt)
+    _check(core().ie_history_append(counts.data_ptr(), seen.data_ptr(), tokens.data_ptr(), slots.data_ptr(),
+                                    None if starts is None else starts.data_ptr(), None if n_prompt is None else n_prompt.data_ptr(),
+                                    n, r, n_slots, vocab, _stream()), what)
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -1176,43 +1197,62 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, slots: torch.Tensor |
     Masks (both or none): row i may only be a token whose bit is set in row ``mask_rows[i]`` (int32 [n]; outside the table: no
     mask) of ``masks`` (int32 [m, ceil(vocab / 32)], bit t % 32 of word t / 32); every other token's logit becomes -inf."""
     what = "adjust_logits"
-    _need(logits.dim() == 2 and logits.shape == out.shape and logits.stride(1) == 1 and out.stride(1) == 1, what,
-          "logits and out are [n, vocab] with adjacent columns")
+    if logits.dim() != 2 or logits.shape != out.shape or logits.stride(1) != 1 or out.stride(1) != 1:
+        _refuse(what, "logits and out are [n, vocab] with adjacent columns")
     n, vocab = logits.shape
-    _need(out.dtype is torch.float32, what, "out is float32")
-    _need(n < 2 or (logits.stride(0) >= vocab and out.stride(0) >= vocab), what, "rows overlap")
-    same = (logits.data_ptr() == out.data_ptr() and logits.dtype is out.dtype and (n < 2 or logits.stride(0) == out.stride(0)))
-    _need(same or not _overlap(logits, out), what, "out shares memory with logits without being logits")
-    words = -(-vocab // 32)
+    code = _CODES.get(logits.dtype)
+    if out.dtype is not _F32 or code is None:
+        _refuse(what, "out is float32, logits float32 or bfloat16")
+    ld_in, ld_out = logits.stride(0), out.stride(0)
+    if n > 1 and (ld_in < vocab or ld_out < vocab):
+        _refuse(what, "rows overlap")
+    at, to = logits.data_ptr(), out.data_ptr()
+    same = at == to and code == IE_F32 and (n < 2 or ld_in == ld_out)
+    if not same and _overlap(logits, out):
+        _refuse(what, "out shares memory with logits without being logits")
+    dev = _here(logits)
+    if out.get_device() != dev:
+        dev = -2
     n_slots = n_bias = n_masks = 0
+    p_slots = p_pen = p_counts = p_seen = p_start = p_ids = p_values = p_rows = p_masks = None
     if slots is not None or penalties is not None or counts is not None or seen is not None:
-        _need(slots is not None and penalties is not None and counts is not None and seen is not None, what,
-              "penalties need slots, penalties, counts and seen")
+        if slots is None or penalties is None or counts is None or seen is None:
+            _refuse(what, "penalties need slots, penalties, counts and seen")
         n_slots, v = _history(what, counts, seen)
-        _need(v == vocab, what, "the history has another vocabulary")
-        _need(slots.shape == (n,) and _ints(slots), what, "slots is a contiguous int32 [n]")
-        _need(penalties.shape == (n, 3) and penalties.dtype is torch.float32 and penalties.is_contiguous(), what,
-              "penalties is a contiguous float32 [n, 3]")
+        if v != vocab:
+            _refuse(what, "the history has another vocabulary")
+        if slots.shape != (n,) or slots.dtype is not _I32 or not slots.is_contiguous():
+            _refuse(what, "slots is a contiguous int32 [n]")
+        if penalties.shape != (n, 3) or penalties.dtype is not _F32 or not penalties.is_contiguous():
+            _refuse(what, "penalties is a contiguous float32 [n, 3]")
+        if not dev == slots.get_device() == penalties.get_device() == counts.get_device() == seen.get_device():
+            dev = -2
+        p_slots, p_pen, p_counts, p_seen = slots.data_ptr(), penalties.data_ptr(), counts.data_ptr(), seen.data_ptr()
     if bias_start is not None or bias_ids is not None or bias_values is not None:
-        _need(bias_start is not None and bias_ids is not None and bias_values is not None, what,
-              "biases need bias_start, bias_ids and bias_values")
-        n_bias = bias_ids.shape[0]
-        _need(bias_start.shape == (n + 1,) and _ints(bias_start) and bias_ids.dim() == 1 and _ints(bias_ids), what,
-              "bias_start is a contiguous int32 [n + 1], bias_ids a contiguous int32 vector")
-        _need(bias_values.shape == (n_bias,) and bias_values.dtype is torch.float32 and bias_values.is_contiguous(), what,
-              "bias_values is a contiguous float32 vector like bias_ids")
+        if bias_start is None or bias_ids is None or bias_values is None:
+            _refuse(what, "biases need bias_start, bias_ids and bias_values")
+        if (bias_start.shape != (n + 1,) or bias_start.dtype is not _I32 or not bias_start.is_contiguous() or bias_ids.dim() != 1
+                or bias_ids.dtype is not _I32 or not bias_ids.is_contiguous()):
+            _refuse(what, "bias_start is a contiguous int32 [n + 1], bias_ids a contiguous int32 vector")
+        if bias_values.shape != bias_ids.shape or bias_values.dtype is not _F32 or not bias_values.is_contiguous():
+            _refuse(what, "bias_values is a contiguous float32 vector like bias_ids")
+        if not dev == bias_start.get_device() == bias_ids.get_device() == bias_values.get_device():
+            dev = -2
+        n_bias, p_start, p_ids, p_values = bias_ids.shape[0], bias_start.data_ptr(), bias_ids.data_ptr(), bias_values.data_ptr()
     if mask_rows is not None or masks is not None:
-        _need(mask_rows is not None and masks is not None, what, "masks need mask_rows and masks")
-        _need(mask_rows.shape == (n,) and _ints(mask_rows), what, "mask_rows is a contiguous int32 [n]")
-        _need(masks.dim() == 2 and masks.shape[1] == words and _ints(masks), what,
-              "masks is a contiguous int32 [m, ceil(vocab / 32)]")
-        n_masks = masks.shape[0]
-    _here(what, logits=logits, out=out, slots=slots, penalties=penalties, counts=counts, seen=seen, bias_start=bias_start,
-          bias_ids=bias_ids, bias_values=bias_values, mask_rows=mask_rows, masks=masks)
-    _check(core().ie_adjust_logits(logits.data_ptr(), dtype_code(logits.dtype), out.data_ptr(), _ptr(slots), _ptr(penalties),
-                                   _ptr(counts), _ptr(seen), _ptr(bias_start), _ptr(bias_ids), _ptr(bias_values), _ptr(mask_rows),
-                                   _ptr(masks), n, vocab, logits.stride(0), out.stride(0), n_slots, n_bias, n_masks,
-                                   1 if same else 0, _stream()), what)
+        if mask_rows is None or masks is None:
+            _refuse(what, "masks need mask_rows and masks")
+        if mask_rows.shape != (n,) or mask_rows.dtype is not _I32 or not mask_rows.is_contiguous():
+            _refuse(what, "mask_rows is a contiguous int32 [n]")
+        if masks.dim() != 2 or masks.shape[1] != (vocab + 31) // 32 or masks.dtype is not _I32 or not masks.is_contiguous():
+            _refuse(what, "masks is a contiguous int32 [m, ceil(vocab / 32)]")
+        if not dev == mask_rows.get_device() == masks.get_device():
+            dev = -2
+        n_masks, p_rows, p_masks = masks.shape[0], mask_rows.data_ptr(), masks.data_ptr()
+    if dev < 0:
+        _away(what, logits, out, slots, penalties, counts, seen, bias_start, bias_ids, bias_values, mask_rows, masks)
+    _check(core().ie_adjust_logits(at, code, to, p_slots, p_pen, p_counts, p_seen, p_start, p_ids, p_values, p_rows, p_masks, n, vocab,
+                                   ld_in, ld_out, n_slots, n_bias, n_masks, 1 if same else 0, _stream()), what)
 
 
 # ------------------------------------------------- tensor-core attention (bfloat16)
@@ -1786,12 +1826,12 @@ _fp8_lib = None
 def fp8_library():
     global _fp8_lib
     if _fp8_lib is None:
-        lib = load_library("fp8", ["fp8_quantize.cu", "gemm_fp8.cu"], dict(BUILD_DEFINES.get("fp8", {})))
+        lib = load_library("fp8", ["fp8_quantize.cu", "gemm_fp8.cu"], dict(BUILD_DEFINES.get("fp8", {})), ["fp8_codes.cuh"])
         P, I, L = c_void_p, c_int, c_longlong
         lib.ie_fp8_quantize_rows.argtypes = [P, I, P, P, I, I, L, L, L, L, P]
         lib.ie_fp8_quantize_blocks.argtypes = [P, I, P, P, I, I, L, L, P]
         lib.ie_gemm_fp8.argtypes = [P, I, P, P, P, P, I, I, I, I, L, L, L, L, L, P, P]
-        lib.ie_gemm_fp8_scratch.argtypes = [I, I]
+        lib.ie_gemm_fp8_scratch.argtypes = [I, I, I, I]
         for name in ("ie_fp8_quantize_rows", "ie_fp8_quantize_blocks", "ie_gemm_fp8"):
             getattr(lib, name).restype = c_int
         lib.ie_gemm_fp8_scratch.restype = c_longlong
@@ -1810,15 +1850,25 @@ def fp8_empty(rows: int, cols: int, device) -> torch.Tensor:
     return torch.empty((rows, max(16, -(-cols // 16) * 16)), dtype=FP8, device=device)[:, :cols]
 
 
-def _codes(what: str, name: str, t: torch.Tensor) -> None:
-    _need(t.dim() == 2 and t.dtype is FP8, what, f"{name} is a float8_e4m3fn matrix")
-    _need((t.stride(1) == 1 or t.shape[1] < 2) and t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0, what,
-          f"rows of {name} are adjacent codes and start on 16 bytes")
+def _codes(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, columns, bytes from row to row) of a matrix of codes."""
+    if t.dim() != 2 or t.dtype is not FP8:
+        _refuse(what, f"{name} is a float8_e4m3fn matrix")
+    rows, cols = t.shape
+    pitch, step = t.stride()
+    if (step != 1 and cols > 1) or pitch % 16 or pitch < cols or t.data_ptr() % 16:
+        _refuse(what, f"rows of {name} are adjacent codes and start on 16 bytes")
+    return rows, cols, pitch
 
 
-def _rows_in(what: str, name: str, t: torch.Tensor) -> None:
-    _need(t.dim() == 2 and t.dtype in _CODES, what, f"{name} is a float32 or bfloat16 matrix")
-    _need(t.stride(1) == 1 or t.shape[1] < 2, what, f"columns of {name} are adjacent")
+def _rows_in(what: str, name: str, t: torch.Tensor) -> int:
+    """The dtype code of a matrix of numbers."""
+    code = _CODES.get(t.dtype)
+    if t.dim() != 2 or code is None:
+        _refuse(what, f"{name} is a float32 or bfloat16 matrix")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        _refuse(what, f"columns of {name} are adjacent")
+    return code
 
 
 def fp8_quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
@@ -1827,66 +1877,78 @@ def fp8_quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
     A scale is the least power of two that brings the group's largest finite number to at most 448 (1 for zeros); a code is
     the nearest e4m3 number to x / scale, ties to even, NaN for a number that is not finite."""
     what = "fp8_quantize_rows"
-    _rows_in(what, "x", x)
-    _codes(what, "codes", codes)
-    n, k = x.shape
-    _need(codes.shape == x.shape, what, "codes has another shape than x")
-    _need(scales.shape == (n, -(-k // FP8_GROUP)) and scales.dtype is torch.float32, what, "scales is float32 [n, ceil(k / 128)]")
-    _here(what, x=x, codes=codes, scales=scales)
-    _check(fp8_library().ie_fp8_quantize_rows(x.data_ptr(), _CODES[x.dtype], codes.data_ptr(), scales.data_ptr(), n, k, x.stride(0),
-                                              codes.stride(0), scales.stride(0), scales.stride(1), _stream()), what)
+    code = _rows_in(what, "x", x)
+    n, k, pitch = _codes(what, "codes", codes)
+    if x.shape != codes.shape:
+        _refuse(what, "codes has another shape than x")
+    if scales.shape != (n, (k + 127) // 128) or scales.dtype is not _F32:
+        _refuse(what, "scales is float32 [n, ceil(k / 128)]")
+    if not _here(x) == codes.get_device() == scales.get_device():
+        _away(what, x, codes, scales)
+    s_row, s_col = scales.stride()
+    _check(fp8_library().ie_fp8_quantize_rows(x.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), n, k, x.stride(0), pitch, s_row,
+                                              s_col, _stream()), what)
 
 
 def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
     """The same for a weight: a scale for each block of 128 rows x 128 columns, ``scales`` contiguous
     [ceil(n / 128), ceil(k / 128)]."""
     what = "fp8_quantize_blocks"
-    _rows_in(what, "w", w)
-    _codes(what, "codes", codes)
-    n, k = w.shape
-    _need(codes.shape == w.shape, what, "codes has another shape than w")
-    _need(scales.shape == (-(-n // FP8_GROUP), -(-k // FP8_GROUP)) and scales.dtype is torch.float32 and scales.is_contiguous(), what,
-          "scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
-    _here(what, w=w, codes=codes, scales=scales)
-    _check(fp8_library().ie_fp8_quantize_blocks(w.data_ptr(), _CODES[w.dtype], codes.data_ptr(), scales.data_ptr(), n, k, w.stride(0),
-                                                codes.stride(0), _stream()), what)
+    code = _rows_in(what, "w", w)
+    n, k, pitch = _codes(what, "codes", codes)
+    if w.shape != codes.shape:
+        _refuse(what, "codes has another shape than w")
+    if scales.shape != ((n + 127) // 128, (k + 127) // 128) or scales.dtype is not _F32 or not scales.is_contiguous():
+        _refuse(what, "scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
+    if not _here(w) == codes.get_device() == scales.get_device():
+        _away(what, w, codes, scales)
+    _check(fp8_library().ie_fp8_quantize_blocks(w.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), n, k, w.stride(0), pitch,
+                                                _stream()), what)
 
 
 def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, x_scales: torch.Tensor | None = None) -> None:
     """out (float32 or bfloat16 [m, n]) = x w^T in 8-bit floating point.  ``w`` (codes, [n, k]) with ``w_scales`` (float32, contiguous,
     [ceil(n / 128), ceil(k / 128)], any positive numbers); ``x`` codes with ``x_scales`` (float32 [m, ceil(k / 128)], any strides), or
     float32 / bfloat16 rows, which are quantised as ``fp8_quantize_rows`` does.  Codes lie as ``fp8_empty`` lays them out.  Sums are
-    float32: inside a block of 128 columns on the tensor cores, over the scaled blocks in registers."""
+    float32: inside a block of 128 columns on the tensor cores, over the scaled blocks in registers.  ``out`` shares no memory with
+    the operands."""
     what = "gemm_fp8"
-    _codes(what, "w", w)
-    n, k = w.shape
+    n, k, w_pitch = _codes(what, "w", w)
+    if x.dim() != 2 or x.shape[1] != k or out.shape != (x.shape[0], n):
+        _refuse(what, "x is [m, k], w [n, k], out [m, n]")
     m = x.shape[0]
-    _need(x.dim() == 2 and x.shape[1] == k and out.shape == (m, n), what, "x is [m, k], w [n, k], out [m, n]")
-    _need(out.dtype in _CODES and (out.stride(1) == 1 or n < 2) and (m < 2 or out.stride(0) >= n), what,
-          "out is a float32 or bfloat16 matrix of adjacent columns")
-    kb = -(-k // FP8_GROUP)
-    _need(w_scales.shape == (-(-n // FP8_GROUP), kb) and w_scales.dtype is torch.float32 and w_scales.is_contiguous(), what,
-          "w_scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
-    _need(k > 0, what, "k is 0")
-    scratch = None
+    to = _CODES.get(out.dtype)
+    ldy = out.stride(0)
+    if to is None or (out.stride(1) != 1 and n > 1) or (m > 1 and ldy < n):
+        _refuse(what, "out is a float32 or bfloat16 matrix of adjacent columns")
+    if w_scales.shape != ((n + 127) // 128, (k + 127) // 128) or w_scales.dtype is not _F32 or not w_scales.is_contiguous():
+        _refuse(what, "w_scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
+    if k == 0:
+        _refuse(what, "k is 0")
+    dev = _here(x)
+    if not dev == w.get_device() == w_scales.get_device() == out.get_device():
+        dev = -2
+    scales, s_row, s_col = None, 0, 0
     if x.dtype is FP8:
-        _codes(what, "x", x)
-        _need(x_scales is not None and x_scales.shape == (m, kb) and x_scales.dtype is torch.float32, what,
-              "codes of x come with x_scales, float32 [m, ceil(k / 128)]")
-        code, s_row, s_col = IE_E4M3, x_scales.stride(0), x_scales.stride(1)
+        code, ldx = IE_E4M3, _codes(what, "x", x)[2]
+        if x_scales is None or x_scales.shape != (m, (k + 127) // 128) or x_scales.dtype is not _F32:
+            _refuse(what, "codes of x come with x_scales, float32 [m, ceil(k / 128)]")
+        if x_scales.get_device() != dev:
+            dev = -2
+        scales, (s_row, s_col) = x_scales.data_ptr(), x_scales.stride()
     else:
-        _rows_in(what, "x", x)
-        _need(x_scales is None, what, "x_scales go with codes of x")
-        code, s_row, s_col = _CODES[x.dtype], 0, 0
-    _here(what, x=x, w=w, w_scales=w_scales, out=out, x_scales=x_scales)
+        code, ldx = _rows_in(what, "x", x), x.stride(0)
+        if x_scales is not None:
+            _refuse(what, "x_scales go with codes of x")
+    if dev < 0:
+        _away(what, x, w, w_scales, out, x_scales)
     if m == 0 or n == 0:
         return
     lib = fp8_library()
-    if code != IE_E4M3:
-        scratch = torch.empty(lib.ie_gemm_fp8_scratch(m, k), dtype=torch.uint8, device=x.device)
-    _check(lib.ie_gemm_fp8(x.data_ptr(), code, _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), _CODES[out.dtype],
-                           m, n, k, x.stride(0), s_row, s_col, w.stride(0), out.stride(0), _ptr(scratch), _stream()), what)
-
+    need = lib.ie_gemm_fp8_scratch(code, m, n, k) if code != IE_E4M3 else 0
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _check(lib.ie_gemm_fp8(x.data_ptr(), code, scales, w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), to, m, n, k, ldx, s_row, s_col,
+                           w_pitch, ldy, None if scratch is None else scratch.data_ptr(), _stream()), what)
 
 
 def attention_tcgen05_library():
