@@ -36,8 +36,15 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--top-p", type=float, default=0.9)
     p.add_argument("--top-k", type=int, default=50)
     p.add_argument("--repetition-penalty", type=float, default=1.0)
+    p.add_argument("--repetition-scope", choices=["window", "history"], default="window",
+                   help="what the repetition penalty goes over: the last 256 generated tokens, or the prompt and all of them")
+    p.add_argument("--presence-penalty", type=float, default=0.0, help="taken off the logit of every token generated before")
+    p.add_argument("--frequency-penalty", type=float, default=0.0, help="taken off once more for each time it was generated")
+    p.add_argument("--logit-bias", default=None, help="added to single tokens' logits: ID:NUMBER,ID:NUMBER,...")
     p.add_argument("--seed", type=int, default=0, help="sampling seed")
     p.add_argument("--dtype", choices=["bfloat16", "float32", "bf16", "fp32"], default="bfloat16")
+    p.add_argument("--weights", choices=["fp8"], default=None,
+                   help="keep the layers' matrices in 8-bit floating point (with --dtype bfloat16)")
     p.add_argument("--device", default="cuda:0")
     p.add_argument("--max-ctx", type=int, default=None, help="size the cache pool for this many tokens")
     p.add_argument("--n-total-blocks", type=int, default=None, help="pages in the cache pool")
@@ -58,6 +65,12 @@ def build_parser() -> argparse.ArgumentParser:
 
 def _parse_ids(text: str) -> list[list[int]]:
     return [[int(t) for t in part.replace(" ", "").split(",") if t] for part in text.split(";") if part.strip()]
+
+
+def _parse_bias(text: str | None) -> dict[int, float] | None:
+    if not text:
+        return None
+    return {int(t): float(v) for t, v in (part.split(":") for part in text.split(",") if part)}
 
 
 def main(argv=None) -> int:
@@ -96,7 +109,7 @@ def main(argv=None) -> int:
         per = args.max_ctx or longest
         n_blocks = -(-per // args.block_size) * min(len(prompts), args.max_batch)
     kw = dict(dtype=args.dtype, device=args.device, n_total_blocks=n_blocks, block_size=args.block_size,
-              max_requests=args.max_batch, eos_token=args.eos_id, max_tokens_per_step=args.max_tokens_per_step,
+              max_requests=args.max_batch, weights=args.weights, eos_token=args.eos_id, max_tokens_per_step=args.max_tokens_per_step,
               chunk=args.chunk, trace_path=args.trace_jsonl, nvtx=args.nvtx)
     if args.checks:
         from .. import kernels
@@ -111,7 +124,9 @@ def main(argv=None) -> int:
         return 2
     t_load = time.perf_counter() - t0
     sampling = SamplingConfig(mode=args.mode, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
-                              repetition_penalty=args.repetition_penalty, seed=args.seed)
+                              repetition_penalty=args.repetition_penalty, seed=args.seed, repetition_scope=args.repetition_scope,
+                              presence_penalty=args.presence_penalty, frequency_penalty=args.frequency_penalty,
+                              logit_bias=_parse_bias(args.logit_bias))
     requests = [Request(req_id=i, prompt_ids=p, max_new_tokens=args.n, sampling=sampling) for i, p in enumerate(prompts)]
     t0 = time.perf_counter()
     out = engine.run_offline(requests)

@@ -19,6 +19,7 @@ import torch
 
 from .. import kernels
 from ..config.registry import detect_config, get_preset
+from ..sampling.history import Adjuster, allowed_words
 from ..sampling.sampler import Sampler, SamplingConfig, pack_rows, request_key
 from ..weights.random_init import write_random_model
 from .batch import StepEntry
@@ -41,6 +42,7 @@ class Engine:
                                    max_tokens_per_step=max_tokens_per_step, chunk=chunk,
                                    max_queue_depth=max_queue_depth, eos_token=eos_token)
         self.sampler = Sampler(runner.rt)
+        self.adjuster = Adjuster(runner.rt, runner.cache.max_requests, runner.spec.vocab_size)
         self.stats = {"steps": 0, "prefill_tokens": 0, "decode_tokens": 0, "preemptions": 0}
         # One step ahead: a step is enqueued before the host has read the tokens of the step before; it
         # takes them on the device.  The host's work for a step then hides behind the GPU's work.
@@ -71,9 +73,10 @@ class Engine:
     # ------------------------------------------------------------ construction
     @classmethod
     def from_dir(cls, model_dir: str | Path, dtype="bfloat16", device="cuda:0", n_total_blocks: int = 4096,
-                 block_size: int = 16, max_requests: int = 64, **kw) -> "Engine":
+                 block_size: int = 16, max_requests: int = 64, weights: str | None = None, **kw) -> "Engine":
+        """``weights="fp8"``: the matrices of the layers are kept in 8-bit floating point (``ModelRunner``)."""
         runner = ModelRunner.from_dir(model_dir, dtype=dtype, device=device, page_size=block_size,
-                                      n_pages=n_total_blocks, max_requests=max_requests)
+                                      n_pages=n_total_blocks, max_requests=max_requests, weights=weights)
         return cls(runner, **kw)
 
     @classmethod
@@ -88,6 +91,15 @@ class Engine:
 
     # ------------------------------------------------------------------ queue
     def submit(self, req: Request) -> bool:
+        if req.sampling is not None and req.sampling.adjusts:
+            try:
+                req.sampling.validate()
+            except ValueError as e:
+                req.error = str(e)
+                return False
+            if any(t >= self.runner.spec.vocab_size for t in req.sampling.logit_bias or ()):
+                req.error = f"logit_bias names a token outside the vocabulary of {self.runner.spec.vocab_size}"
+                return False
         if not req.arrival_time:
             req.arrival_time = time.perf_counter()      # the clock that run_offline and generate step with
         return self.scheduler.submit(req)
@@ -131,15 +143,32 @@ class Engine:
             if self._nvtx:
                 torch.cuda.nvtx.range_pop()
 
-    # a penalty over generated tokens needs them on the host; so does a plan that may have to preempt
+    # a penalty over the last generated tokens needs them on the host; so do a mask of allowed tokens, a history that has to be written
+    # anew, and a plan that may have to preempt
     def _can_pipeline(self) -> bool:
         s = self.scheduler
-        if self.cfg.repetition_penalty != 1.0:
+        if self.cfg.windowed:
             return False
         for r in list(s.running) + s.queue[:4]:
-            if r.sampling is not None and r.sampling.repetition_penalty != 1.0:
+            c = r.sampling or self.cfg
+            if c.windowed or r.allowed_tokens is not None:
+                return False
+            if c.keeps_history and r.generated and r.generated[-1] == PLACEHOLDER and not self._history_is_current(r):
                 return False
         return s.cache.n_free_pages() >= len(s.running) + 1
+
+    def _history_is_current(self, r: Request) -> bool:
+        slot = self.runner.cache.slots.get(r.req_id)
+        return slot is not None and self.adjuster.history is not None and self.adjuster.history.current(slot, r)
+
+    def _rows(self, wanted, configs, allowed=None):
+        """The rows as ``Adjuster`` takes them, None when none of them asks for anything."""
+        if not any(c.adjusts for c in {id(c): c for c in configs}.values()) and not (allowed and any(a is not None for a in allowed)):
+            return None
+        slots = self.runner.cache.slots
+        rows = [(e.request, c, slots[e.request.req_id], allowed[i] if allowed else None)
+                for i, (e, c) in enumerate(zip(wanted, configs))]
+        return rows
 
     def _drain(self, now: float) -> list[Request]:
         if self._pending is None:
@@ -175,9 +204,12 @@ class Engine:
         wanted = [e for e in plan.entries if e.wants_logits]
         configs = [e.request.sampling or self.cfg for e in wanted]
         keys = [request_key(e.request.req_id, len(e.request.generated)) for e in wanted]
-        rows = pack_rows(configs, keys, self.runner.spec.vocab_size) if wanted else None
-        _, ids = self.runner.step_and_sample(entries, rows, device_tokens=prev["dev"] if any_src else None,
-                                             token_src=token_src if any_src else None)
+        adjust = self._rows(wanted, configs)
+        rows = pack_rows(configs, keys, self.runner.spec.vocab_size) if wanted and adjust is None else None
+        logits, ids = self.runner.step_and_sample(entries, rows, device_tokens=prev["dev"] if any_src else None,
+                                                  token_src=token_src if any_src else None)
+        if adjust is not None:
+            ids = self.sampler.sample(logits, configs, keys, adjuster=self.adjuster, rows=adjust)
         for e in plan.entries:
             self.stats["decode_tokens" if len(e.tokens) == 1 and e.request.generated else "prefill_tokens"] += len(e.tokens)
         self.stats["steps"] += 1
@@ -207,7 +239,9 @@ class Engine:
         wanted = [e for e in plan.entries if e.wants_logits]
         configs = [e.request.sampling or self.cfg for e in wanted]
         keys = [request_key(e.request.req_id, len(e.request.generated)) for e in wanted]
-        if wanted and all(c.repetition_penalty == 1.0 for c in configs):
+        allowed, stuck = self._allowed(wanted)
+        adjust = self._rows(wanted, configs, allowed)
+        if wanted and adjust is None and not any(c.windowed for c in configs):
             # sampling rides in the step (inside the CUDA graph of a decode step)
             rows = pack_rows(configs, keys, self.runner.spec.vocab_size)
             _, ids = self.runner.step_and_sample(entries, rows)
@@ -216,15 +250,28 @@ class Engine:
             ids = None
             if wanted:
                 contexts = [e.request.generated for e in wanted]
-                ids = self.sampler.sample(logits, configs, keys, contexts)
+                ids = self.sampler.sample(logits, configs, keys, contexts, self.adjuster if adjust else None, adjust)
         if wanted:
             ids = ids.tolist()                                   # the step's one device-to-host read
-            sampled = {e.request.req_id: t for e, t in zip(wanted, ids)}
+            sampled = {e.request.req_id: None if e.request.req_id in stuck else t for e, t in zip(wanted, ids)}
         for e in plan.entries:
             self.stats["decode_tokens" if len(e.tokens) == 1 and e.request.generated else "prefill_tokens"] += len(e.tokens)
         self.stats["steps"] += 1
         self._observe(plan, t_host0, False)
         return self.scheduler.commit(plan, sampled, now)
+
+    def _allowed(self, wanted):
+        """Masks of the rows whose requests hold the next token to a set, and the ids of requests that no token may continue."""
+        allowed, stuck = [], set()
+        for e in wanted:
+            r, words = e.request, None
+            if r.allowed_tokens is not None and (may := r.allowed_tokens(r.generated)) is not None:
+                words = allowed_words(may, self.runner.spec.vocab_size)
+                if not words.any():
+                    stuck.add(r.req_id)
+                    words = None
+            allowed.append(words)
+        return allowed, stuck
 
     def run_offline(self, requests: list[Request]) -> dict[int, list[int]]:
         """Submit everything, run to completion; ``{req_id: generated}``

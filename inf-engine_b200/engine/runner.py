@@ -40,14 +40,26 @@ def parse_dtype(dtype) -> torch.dtype:
 
 class ModelRunner:
     def __init__(self, config, tensors: dict, dtype, device="cuda:0", page_size: int = 16, n_pages: int = 256,
-                 max_requests: int = 64, spec=None, use_graphs: bool = True, poison_free_pages: bool = False):
+                 max_requests: int = 64, spec=None, use_graphs: bool = True, poison_free_pages: bool = False,
+                 weights: str | None = None):
+        """``weights="fp8"``: the layers' matrices (those that multiply a step's rows; not the embedding, the head, and
+        what a mixture's experts hold) are kept in 8-bit floating point with a scale for each block of 128 x 128, and their products
+        quantise the rows as they come (``kernels.gemm_fp8``).  Activations, cache and everything else stay bfloat16."""
         self.config = config
         self.spec = spec if spec is not None else config.model_spec()
         self.dtype = parse_dtype(dtype)
         self.device = torch.device(device)
+        if weights not in (None, "fp8"):
+            raise ValueError(f"weights are kept as they come (None) or as 'fp8', not {weights!r}")
+        if weights and self.dtype is not torch.bfloat16:
+            raise ValueError("weights='fp8' goes with dtype bfloat16")
         torch.cuda.set_device(self.device)
-        self.rt = Runtime(self.device, self.dtype)
+        self.rt = Runtime(self.device, self.dtype, weights)
         self.model = build_model(self.spec, tensors, self.rt)     # the top level that spec.kind names
+        if weights:
+            for layer in getattr(self.model, "layers", ()):
+                if getattr(layer.mixer, "o_weight", None) is not None:
+                    layer.mixer.o_weight = None                   # its product holds the codes
         max_pages_per_request = -(-self.spec.max_positions // page_size)
         self.cache = CacheManager(self.model.cache_requirements(), page_size, n_pages, max_requests,
                                   min(n_pages, max_pages_per_request))

@@ -1906,12 +1906,21 @@ def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
                                                 _stream()), what)
 
 
-def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, x_scales: torch.Tensor | None = None) -> None:
+def gemm_fp8_scratch_bytes(x: torch.Tensor, n: int) -> int:
+    """Bytes that ``gemm_fp8`` needs for the codes of rows ``x`` that it quantises, with a weight of ``n`` rows (0: none)."""
+    if x.dtype is FP8:
+        return 0
+    return int(fp8_library().ie_gemm_fp8_scratch(_CODES[x.dtype], x.shape[0], n, x.shape[1]))
+
+
+def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, x_scales: torch.Tensor | None = None,
+             scratch: torch.Tensor | None = None) -> None:
     """out (float32 or bfloat16 [m, n]) = x w^T in 8-bit floating point.  ``w`` (codes, [n, k]) with ``w_scales`` (float32, contiguous,
     [ceil(n / 128), ceil(k / 128)], any positive numbers); ``x`` codes with ``x_scales`` (float32 [m, ceil(k / 128)], any strides), or
     float32 / bfloat16 rows, which are quantised as ``fp8_quantize_rows`` does.  Codes lie as ``fp8_empty`` lays them out.  Sums are
     float32: inside a block of 128 columns on the tensor cores, over the scaled blocks in registers.  ``out`` shares no memory with
-    the operands."""
+    the operands.  ``scratch`` (uint8, at least ``gemm_fp8_scratch_bytes(x, n)``) takes the codes of rows that are quantised here;
+    without it they go into memory of this call's own."""
     what = "gemm_fp8"
     n, k, w_pitch = _codes(what, "w", w)
     if x.dim() != 2 or x.shape[1] != k or out.shape != (x.shape[0], n):
@@ -1946,7 +1955,13 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
         return
     lib = fp8_library()
     need = lib.ie_gemm_fp8_scratch(code, m, n, k) if code != IE_E4M3 else 0
-    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    if not need:
+        scratch = None
+    elif scratch is None:
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif (scratch.dtype is not torch.uint8 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16
+          or scratch.get_device() != dev):
+        _refuse(what, f"scratch is {need} contiguous bytes that start on 16, beside the operands")
     _check(lib.ie_gemm_fp8(x.data_ptr(), code, scales, w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), to, m, n, k, ldx, s_row, s_col,
                            w_pitch, ldy, None if scratch is None else scratch.data_ptr(), _stream()), what)
 

@@ -7,7 +7,8 @@ Which kernel runs is decided by the dtypes:
   * bfloat16 activations and weight: the library matrix product (cuBLAS through
     ``torch.mm``), which is what the reference's engine uses for every
     projection, or this package's own kernels where they are registered for the
-    shape.
+    shape;
+  * a weight kept in 8-bit floating point (``Runtime.weights``): this package's 8-bit product, whatever the activations.
 """
 
 from __future__ import annotations
@@ -44,6 +45,14 @@ class Linear:
         self.rt = rt
         self.name = name
         self.out_features, self.in_features = weight.shape
+        self.scales = None
+        # a product of fewer than a block of scales each way, such as a gate of a few heads, stays as it is, and so does the head
+        if (getattr(rt, "weights", None) == "fp8" and name != "head" and weight.dtype is torch.bfloat16
+                and min(self.out_features, self.in_features) >= kernels.FP8_GROUP):
+            self.weight = kernels.fp8_empty(self.out_features, self.in_features, weight.device)
+            self.scales = torch.empty((-(-self.out_features // kernels.FP8_GROUP), -(-self.in_features // kernels.FP8_GROUP)),
+                                      dtype=torch.float32, device=weight.device)
+            kernels.fp8_quantize_blocks(weight, self.weight, self.scales)
         assert bias is None or tuple(bias.shape) == (self.out_features,)
         self.bias = bias.contiguous() if bias is not None else None
 
@@ -79,6 +88,10 @@ class Linear:
         w = self.weight
         assert x.shape[1] == self.in_features and out.shape == (x.shape[0], self.out_features)
         if x.shape[0] == 0:
+            return out
+        if self.scales is not None:
+            n = kernels.gemm_fp8_scratch_bytes(x, self.out_features)
+            kernels.gemm_fp8(x, w, self.scales, out, scratch=self.rt.ws.take("fp8_rows", (n,), torch.uint8) if n else None)
             return out
         if x.dtype is torch.float32 or w.dtype is torch.float32:
             kernels.gemm_simt(x, w, out)

@@ -91,8 +91,9 @@ class Staging:
 
 
 class Runtime:
-    def __init__(self, device: str | torch.device, act_dtype: torch.dtype):
+    def __init__(self, device: str | torch.device, act_dtype: torch.dtype, weights: str | None = None):
         self.device = torch.device(device)
+        self.weights = weights      # how ``Linear`` keeps its matrix: None as it comes, "fp8" in 8-bit floating point
         if self.device.type != "cuda":
             raise RuntimeError("the engine runs on a CUDA device only; there is no CPU path")
         if act_dtype not in (torch.float32, torch.bfloat16):

@@ -1,3 +1,4 @@
+from .history import Adjuster, TokenHistory, allowed_words
 from .sampler import (
     REPETITION_PENALTY_WINDOW,
     Sampler,

@@ -12,6 +12,7 @@ Differences that are on purpose:
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from enum import Enum
 
@@ -33,7 +34,12 @@ class SamplingMode(str, Enum):
 
 @dataclass
 class SamplingConfig:
-    """Decoding options; names and defaults as engine/sampling.py:24-47, plus ``seed``."""
+    """Decoding options; names and defaults as engine/sampling.py:24-47, plus ``seed`` and what is below it.
+
+    ``repetition_scope``: the repetition penalty goes over the last 256 generated tokens (``"window"``, the reference's), or over the
+    prompt and everything generated (``"history"``).  ``presence_penalty`` is taken off the logit of every token generated before,
+    ``frequency_penalty`` once more for each time.  ``logit_bias`` adds to the logits of single tokens ({token id: number}).  They
+    come in this order, before temperature, top-k and top-p."""
 
     mode: SamplingMode = SamplingMode.GREEDY
     temperature: float = 1.0
@@ -41,9 +47,28 @@ class SamplingConfig:
     top_p: float = 0.9
     repetition_penalty: float = 1.0
     seed: int = 0
+    repetition_scope: str = "window"
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: dict[int, float] | None = None
 
     def __post_init__(self):
         self.mode = SamplingMode(self.mode)
+
+    @property
+    def windowed(self) -> bool:
+        """Whether the penalty over the last generated tokens is asked for, which needs them on the host."""
+        return self.repetition_penalty != 1.0 and self.repetition_scope == "window"
+
+    @property
+    def keeps_history(self) -> bool:
+        """Whether a penalty is asked for that reads what the request has said from the device."""
+        return (self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+                or (self.repetition_penalty != 1.0 and self.repetition_scope == "history"))
+
+    @property
+    def adjusts(self) -> bool:
+        return self.keeps_history or bool(self.logit_bias)
 
     def validate(self) -> None:
         if self.mode is not SamplingMode.GREEDY and self.temperature <= 0.0:
@@ -52,6 +77,16 @@ class SamplingConfig:
             raise ValueError("top_p must be in (0, 1]")                      # engine/sampling.py:167-168
         if self.repetition_penalty <= 0.0:
             raise ValueError("repetition_penalty must be positive")
+        if self.repetition_scope not in ("window", "history"):
+            raise ValueError("repetition_scope must be 'window' or 'history'")
+        for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
+            if not math.isfinite(getattr(self, name)):
+                raise ValueError(f"{name} must be finite")
+        for t, v in (self.logit_bias or {}).items():
+            if isinstance(t, bool) or not isinstance(t, (int, np.integer)) or t < 0:
+                raise ValueError(f"logit_bias maps token ids to numbers, not {t!r}")
+            if not math.isfinite(v) or abs(v) > 1e30:
+                raise ValueError(f"the bias of token {t} must be finite (1e30 at most)")
 
 
 def splitmix64(x: int) -> int:
@@ -98,17 +133,18 @@ class Sampler:
         self.rt = rt
 
     def sample(self, logits: torch.Tensor, configs: list[SamplingConfig], keys: list[int],
-               contexts: list[list[int]] | None = None) -> torch.Tensor:
+               contexts: list[list[int]] | None = None, adjuster=None, rows=None) -> torch.Tensor:
         """One token per row of float32 ``logits`` [M, V] -> int32 [M] on the device.
 
         ``contexts[i]`` (tokens seen so far) matters only to rows with a repetition
         penalty; the penalty rewrites the logits in place, as the reference's does on
-        a copy (engine/sampling.py:120).
+        a copy (engine/sampling.py:120).  With ``adjuster`` and ``rows`` (``history.Adjuster``) the logits are adjusted in place,
+        and the tokens go into the histories of the rows that keep one.
         """
         m, vocab = logits.shape
         assert len(configs) == m and len(keys) == m
         out = self.rt.ws.take("sampled", (m,), torch.int32)
-        pens = [c.repetition_penalty for c in configs]
+        pens = [c.repetition_penalty if c.windowed else 1.0 for c in configs]
         if contexts is not None and any(p != 1.0 for p in pens):
             w = REPETITION_PENALTY_WINDOW
             ctx = np.full((m, w), -1, dtype=np.int32)
@@ -119,10 +155,12 @@ class Sampler:
             pen = np.asarray(pens, dtype=np.float32).view(np.int32)
             dev = self.rt.staging.upload(np.concatenate([ctx.reshape(-1), pen]))
             kernels.repetition_penalty(logits, dev[:m * w].view(m, w), dev[m * w:].view(torch.float32))
+        kept = adjuster.apply(logits, rows) if adjuster is not None else None
         if all(c.mode is SamplingMode.GREEDY for c in configs):
             kernels.argmax(logits, out)
-            return out
-        rows = pack_rows(configs, keys, vocab)
-        dev = self.rt.staging.upload(rows.reshape(-1)).view(m, 7)
-        kernels.sample(logits, dev, out)
+        else:
+            dev = self.rt.staging.upload(pack_rows(configs, keys, vocab).reshape(-1)).view(m, 7)
+            kernels.sample(logits, dev, out)
+        if kept is not None:
+            adjuster.history.record(out, *kept)
         return out
