@@ -13,6 +13,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 enum { IE_E4M3 = 2 };      // dtype code of an operand that is quantised already
+#define IE_NEEDS_SCRATCH -5  /* the rows are to be quantised, and there is no room for their codes */
 
 struct Fp8Params {
   const uint8_t* x;
@@ -446,6 +447,220 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
   }
 }
 
+// ------------------------------------------------------------------- a long weight under few rows
+// Up to 32 rows of x: the weight's bytes are the bound, and it is the MMA's larger operand: 128 rows of w by TX rows of x a tile, a block
+// of K a stage.  Nothing converts a code (on the matrix instructions for halves, the conversions of both operands take 96 cycles of an
+// SM for 2 KB of the weight, which memory brings in 85), the ring holds 9 or 10 stages of 16 KB, and with TX columns a sum the tensor
+// memory holds four blocks' sums, so the trip from MMA to summing warps and back is not waited for.  One scale of w holds for a
+// whole tile, those of x go by columns.  SPLIT as above: the blocks of a cluster share a tile.
+constexpr int THIN_THREADS = 256, THIN_SUMS = 4, THIN_LEAST = 4;       // TMA, MMA, two that do nothing, four that sum
+template <int TX> constexpr int THIN_STAGE = (128 + TX) * GROUP;
+template <int TX> constexpr int THIN_STAGES = TX == 16 ? 10 : 9;
+template <int TX> constexpr int THIN_SMEM = 1024 + THIN_STAGES<TX> * THIN_STAGE<TX>;
+
+template <int TX, bool SPLIT>
+__global__ void __launch_bounds__(THIN_THREADS, 1) gemm_fp8_thin_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                                        const __grid_constant__ CUtensorMap map_w, Fp8Params p) {
+  constexpr int NS = THIN_STAGES<TX>, BYTES = THIN_STAGE<TX>, W_BYTES = 128 * GROUP, PITCH = 132;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ __align__(8) unsigned long long bars[2 * NS + 2 * THIN_SUMS];     // full, empty, acc_full, acc_empty
+  __shared__ __align__(16) float scales[4][AHEAD][TX + 4];                     // of each summing warp: of x, then that of w
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int failed;
+  static_assert(TX * PITCH * 4 <= NS * BYTES, "the sums of a split tile fit the ring");
+
+  pdl_trigger();
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const uint32_t ring = (saddr(smem_raw) + 1023u) & ~1023u;
+  unsigned char* ring_ptr = smem_raw + (ring - saddr(smem_raw));
+  const uint32_t full0 = saddr(&bars[0]), empty0 = saddr(&bars[NS]), acc_full0 = saddr(&bars[2 * NS]), acc_empty0 = acc_full0 + 8 * THIN_SUMS;
+  const int k_blocks = (p.K + GROUP - 1) / GROUP, tiles = (p.N + 127) / 128;
+  const int rank = SPLIT ? (int)(blockIdx.x % p.split) : 0;
+  const int t0 = SPLIT ? (int)(blockIdx.x / p.split) : (int)blockIdx.x, t_step = SPLIT ? tiles : (int)gridDim.x;
+  const int kb0 = SPLIT ? k_blocks * rank / p.split : 0, kb1 = SPLIT ? k_blocks * (rank + 1) / p.split : k_blocks;
+
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
+    failed = 0;
+    for (int s = 0; s < NS; ++s) {
+      bar_init(full0 + 8 * s, 1);
+      bar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < THIN_SUMS; ++b) {
+      bar_init(acc_full0 + 8 * b, 1);
+      bar_init(acc_empty0 + 8 * b, 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_slot)), "n"(THIN_SUMS * TX) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    int s = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const int ahead = p.early ? min(NS, kb1 - kb0) : 0;              // the ring's first round of the weight, before x is there
+    if (elect_one()) {
+      for (int i = 0; i < ahead; ++i) {
+        bar_expect(full0 + 8 * i, BYTES);
+        tma_load<false>(ring + i * BYTES, &map_w, (kb0 + i) * GROUP, t0 * 128, full0 + 8 * i);
+      }
+    }
+    __syncwarp();
+    pdl_wait();
+    for (int t = t0; t < tiles && ok; t += t_step) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = __all_sync(0xffffffffu, bar_wait(empty0 + 8 * s, phase ^ 1, &failed));
+        if (!ok) { atomicExch(&g_fp8_error, 5); failed = 1; break; }
+        const bool asked = t == t0 && kb - kb0 < ahead;
+        if (elect_one()) {
+          if (!asked) {
+            bar_expect(full0 + 8 * s, BYTES);
+            tma_load<false>(ring + s * BYTES, &map_w, kb * GROUP, t * 128, full0 + 8 * s);
+          }
+          tma_load<false>(ring + s * BYTES + W_BYTES, &map_x, kb * GROUP, 0, full0 + 8 * s);
+        }
+        __syncwarp();
+        if (++s == NS) { s = 0; phase ^= 1; }
+      }
+    }
+    if (failed) for (int i = 0; i < 2048; ++i) __nanosleep(64);      // copies under way still land in this block's memory
+  } else if (warp == 1) {
+    int s = 0, buf = 0;
+    uint32_t phase = 0, acc_phase = 1;
+    bool ok = true;
+    for (int t = t0; t < tiles && ok; t += t_step) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = __all_sync(0xffffffffu, bar_wait(acc_empty0 + 8 * buf, acc_phase, &failed));
+        if (!ok) { atomicExch(&g_fp8_error, 6); failed = 1; break; }
+        ok = __all_sync(0xffffffffu, bar_wait(full0 + 8 * s, phase, &failed));
+        if (!ok) { atomicExch(&g_fp8_error, 7); failed = 1; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t a = smem_desc(ring + s * BYTES), b = smem_desc(ring + s * BYTES + W_BYTES);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < GROUP / 32; ++k)
+            mma_fp8<false>(tmem + (uint32_t)(buf * TX), a + 2 * k, b + 2 * k, instr_desc(128, TX), k > 0 ? 1u : 0u);
+          mma_commit<false>(empty0 + 8 * s);
+          mma_commit<false>(acc_full0 + 8 * buf);
+        }
+        __syncwarp();
+        if (++s == NS) { s = 0; phase ^= 1; }
+        if (++buf == THIN_SUMS) { buf = 0; acc_phase ^= 1; }
+      }
+    }
+  } else if (warp >= 4) {
+    const int quarter = warp & 3;                                    // tensor memory lanes, rows of w
+    const uint32_t my_tmem = tmem + ((uint32_t)(quarter * 32) << 16);
+    float (*mine)[TX + 4] = scales[quarter];
+    const uint32_t slots = saddr(&scales[quarter][0][0]);
+    // The scales of a block come AHEAD blocks early, a column of x a lane, on into the next tile
+    int ahead_t = t0, ahead_kb = kb0, ahead_slot = 0;
+    const auto ask = [&]() {
+      if (ahead_t < tiles) {
+        const uint32_t dst = slots + ahead_slot * (TX + 4) * 4;
+        for (int j = lane; j < TX; j += 32)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * j), "l"(p.sx + min(j, p.M - 1) * p.sx_row + ahead_kb * p.sx_col) : "memory");
+        if (lane == 0)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * TX), "l"(p.sw + (long long)ahead_t * k_blocks + ahead_kb) : "memory");
+        if (++ahead_kb == kb1) { ahead_kb = kb0; ahead_t += t_step; }
+      }
+      ahead_slot = (ahead_slot + 1) % AHEAD;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    pdl_wait();                                                      // the scales of x come from the kernel ahead
+    for (int i = 0; i < AHEAD - 1; ++i) ask();
+    int it = 0, buf = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int t = t0; t < tiles && ok; t += t_step) {
+      float acc[TX];
+#pragma unroll
+      for (int j = 0; j < TX; ++j) acc[j] = 0.f;
+#pragma unroll 1
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        __syncwarp();                                                // every lane has read the slot that is filled next
+        ask();
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        __syncwarp();                                                // every lane's copies into this block's slot are there
+        const float* sx = mine[it % AHEAD];
+        const float sw = sx[TX];
+        ok = bar_wait(acc_full0 + 8 * buf, acc_phase, &failed);
+        if (!ok) { atomicExch(&g_fp8_error, 8); failed = 1; }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        uint32_t r[TX / 16][16];
+#pragma unroll
+        for (int c = 0; c < TX / 16; ++c) tmem_ld16(my_tmem + (uint32_t)(buf * TX + 16 * c), r[c]);
+#pragma unroll
+        for (int c = 0; c < TX / 16; ++c) tmem_ld_wait(r[c]);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(acc_empty0 + 8 * buf);
+#pragma unroll
+        for (int j = 0; j < TX; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(sx + j);
+          acc[j] = fmaf(__uint_as_float(r[j / 16][j % 16]), f.x * sw, acc[j]);
+          acc[j + 1] = fmaf(__uint_as_float(r[j / 16][j % 16 + 1]), f.y * sw, acc[j + 1]);
+          acc[j + 2] = fmaf(__uint_as_float(r[j / 16][j % 16 + 2]), f.z * sw, acc[j + 2]);
+          acc[j + 3] = fmaf(__uint_as_float(r[j / 16][j % 16 + 3]), f.w * sw, acc[j + 3]);
+        }
+        if (++buf == THIN_SUMS) { buf = 0; acc_phase ^= 1; }
+      }
+      if (!ok) break;
+      const int row = quarter * 32 + lane;
+      if (SPLIT) {
+        float* part = reinterpret_cast<float*>(ring_ptr);            // the ring is free: every MMA that read it has finished
+#pragma unroll
+        for (int j = 0; j < TX; ++j) part[j * PITCH + row] = acc[j];
+      } else {
+        const int n = t * 128 + row;
+#pragma unroll
+        for (int j = 0; j < TX; ++j)
+          if (j < p.M && n < p.N) {
+            if (p.y_bf16) ((bf16*)p.y)[j * p.ldy + n] = __float2bfloat16_rn(acc[j]);
+            else ((float*)p.y)[j * p.ldy + n] = acc[j];
+          }
+      }
+    }
+  }
+
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (SPLIT) {
+    // every block of the cluster comes here, one whose waits ran out too
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int items = p.M * 32, first = items * rank / p.split, end = items * (rank + 1) / p.split;
+    for (int i = first + tid; i < end; i += THIN_THREADS) {
+      const int m = i / 32, c = i % 32 * 4;
+      float4 v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < p.split) v[q] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(cluster.map_shared_rank(ring_ptr, q)) + m * PITCH + c);
+      float4 s = v[0];
+#pragma unroll
+      for (int q = 1; q < 8; ++q)
+        if (q < p.split) { s.x += v[q].x; s.y += v[q].y; s.z += v[q].z; s.w += v[q].w; }
+      if (t0 * 128 + c < p.N) store4(p, m, t0 * 128 + c, s);
+    }
+    cluster.sync();                                                  // a block's memory is read until here
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(THIN_SUMS * TX) : "memory");
+  }
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -463,13 +678,13 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// codes [rows, cols], row pitch ld bytes: boxes of 128 rows x 128 columns, zeros beyond the last column and row
-int make_map(CUtensorMap* map, const void* base, int rows, int cols, long long ld) {
+// codes [rows, cols], row pitch ld bytes: boxes of `high` rows x 128 columns, zeros beyond the last column and row
+int make_map(CUtensorMap* map, const void* base, int rows, int cols, long long ld, int high = 128) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return IE_BAD_SIZE;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld};
-  const cuuint32_t box[2] = {(cuuint32_t)GROUP, 128};
+  const cuuint32_t box[2] = {(cuuint32_t)GROUP, (cuuint32_t)high};
   const cuuint32_t elem[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -479,29 +694,37 @@ int make_map(CUtensorMap* map, const void* base, int rows, int cols, long long l
 
 constexpr size_t TILE_SMEM = 1024 + STAGES * STAGE + 8 * OUT_STAGE + AHEAD * 256 * 8;
 
-// clusters of `size` blocks of the split form that the current device runs at once
-int clusters_that_fit(int size) {
-  static std::atomic<int> known[64][9];
+// clusters of `size` blocks of a kernel that the current device runs at once; `known`: what was asked before, by device and size
+typedef std::atomic<int> FitTable[64][9];
+int clusters_that_fit(const void* kernel, int threads, int smem, int size, FitTable& known) {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < 64 && (n = known[dev][size].load(std::memory_order_relaxed)) > 0) return n;
-  if (cudaFuncSetAttribute(gemm_fp8_tile_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TILE_SMEM) != cudaSuccess) return 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = size * 1024;
-  cfg.blockDim = TILE_THREADS;
-  cfg.dynamicSmemBytes = TILE_SMEM;
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute a;
   a.id = cudaLaunchAttributeClusterDimension;
   a.val.clusterDim.x = size;
   a.val.clusterDim.y = a.val.clusterDim.z = 1;
   cfg.attrs = &a;
   cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tile_kernel<false, true>, &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
     cudaGetLastError();                                // this size does not fit: nothing that a later launch should report
     return 0;
   }
   if (dev < 64) known[dev][size].store(n, std::memory_order_relaxed);
   return n;
+}
+// As many blocks as can share a tile with all tiles under way at once and `least` blocks of K each
+template <typename Kernel>
+int blocks_a_tile(Kernel kernel, int threads, int smem, long long tiles, int k_blocks, int least, FitTable& known) {
+  int split = 1;
+  for (int s = 2; s <= 8 && least * s <= k_blocks; ++s)
+    if (clusters_that_fit((const void*)kernel, threads, smem, s, known) >= tiles) split = s;
+  return split;
 }
 
 template <bool PAIR, bool SPLIT>
@@ -532,12 +755,35 @@ int launch_tiles(Fp8Params p, int sms, cudaStream_t stream) {
   return launch_k(gemm_fp8_tile_kernel<PAIR, SPLIT>, (unsigned)blocks, TILE_THREADS, SMEM, stream, mx, mw, p);
 }
 
+template <int TX>
+int launch_thin(Fp8Params p, int sms, cudaStream_t stream) {
+  CUtensorMap mx, mw;
+  int rc = make_map(&mx, p.x, p.M, p.K, p.ldx, TX);
+  if (rc) return rc;
+  rc = make_map(&mw, p.w, p.N, p.K, p.ldw);
+  if (rc) return rc;
+  static_assert(THIN_SMEM<TX> <= 232448 - 16 * 1024, "shared memory of a block");
+  static OncePerDevice once;
+  rc = once([] {
+    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_thin_kernel<TX, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, THIN_SMEM<TX>);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(gemm_fp8_thin_kernel<TX, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, THIN_SMEM<TX>);
+  });
+  if (rc) return rc;
+  static FitTable fits;
+  const int tiles = (p.N + 127) / 128;
+  p.split = blocks_a_tile(gemm_fp8_thin_kernel<TX, true>, THIN_THREADS, THIN_SMEM<TX>, tiles, (p.K + GROUP - 1) / GROUP, THIN_LEAST, fits);
+  if (p.split > 1)
+    return launch_k_cluster(gemm_fp8_thin_kernel<TX, true>, p.split, (unsigned)(tiles * p.split), THIN_THREADS, THIN_SMEM<TX>, stream, mx, mw, p);
+  return launch_k(gemm_fp8_thin_kernel<TX, false>, (unsigned)(tiles < sms ? tiles : sms), THIN_THREADS, THIN_SMEM<TX>, stream, mx, mw, p);
+}
+
 // ------------------------------------------------------------------- few rows
-// Up to 16 rows of x (decode steps): the weight's bytes are the bound, so they go from memory straight into the registers that the
-// matrix instruction reads, 16 bytes a lane, a block of K ahead of the one at work.  A warp holds 16 R rows of w, the instruction's
-// larger side, and 8 NT rows of x.  The codes become halves, which hold them exactly (an instruction for e4m3 exists, but is made
-// of the same conversions, of both operands every time).  The instruction wants of lane (g, t) two numbers from 2 t and two from
-// 8 + 2 t of its 16; any other dealing of K serves as well if both operands share it, so lane t takes 16 neighbouring codes of 64,
+// Up to 16 rows of x under a weight that is not long: the weight goes from memory straight into the registers that the matrix
+// instruction reads, 16 bytes a lane, a block of K ahead of the one at work.  A warp holds 16 rows of w, the instruction's larger
+// side, and 8 NT rows of x.  The codes become halves, which hold them exactly (an instruction for e4m3 exists, but is made of the
+// same conversions, of both operands every time; they are what bounds this kernel, so slots in shared memory with more blocks of K
+// ahead do not help: 4 x 8192 x 8192 took 22 us with four, 15.9 so).  The instruction wants of lane (g, t) two numbers from 2 t and two
+// from 8 + 2 t of its 16; any other dealing of K serves as well if both operands share it, so lane t takes 16 neighbouring codes of 64,
 // for four instructions.  ks warps share rows of w and deal out K where there are few rows; their sums come together in shared
 // memory, in the order of K.
 constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32;
@@ -560,6 +806,7 @@ __device__ __forceinline__ uint4 stream_codes(const uint8_t* at) {
   asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
   return v;
 }
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 // four codes -> the first two and the last two as halves
 __device__ __forceinline__ void halves(uint32_t codes, uint32_t& first, uint32_t& last) {
   asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(first), "=r"(last) : "r"(codes));
@@ -619,36 +866,36 @@ __device__ __forceinline__ void quantize_row(const RawRow& r, uint4 (&codes)[2],
 }
 
 // RAW: x comes in bfloat16 and is quantised here (one tile of 8 rows)
-template <int NT, int R, bool RAW>
+template <int NT, bool RAW>
 __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params p, int ks) {
   static_assert(!RAW || NT == 1, "registers for one tile of raw rows");
-  __shared__ float sums[FEW_WARPS][16 * R][8 * NT + 1];
+  __shared__ float sums[FEW_WARPS][16][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int groups = FEW_WARPS / ks, slice = warp % ks, k_blocks = (p.K + GROUP - 1) / GROUP;
-  const int n0 = (blockIdx.x * groups + warp / ks) * 16 * R;
+  const int n0 = (blockIdx.x * groups + warp / ks) * 16;
   const int kb0 = k_blocks * slice / ks, kb1 = n0 < p.N ? k_blocks * (slice + 1) / ks : kb0;
-  const uint8_t* rows[2 * R];
+  const uint8_t* rows[2];
 #pragma unroll
-  for (int i = 0; i < 2 * R; ++i) rows[i] = p.w + (long long)min(n0 + g + 8 * i, p.N - 1) * p.ldw + 16 * t;
-  uint4 w[2][2 * R][2];
-  const auto ask = [&](uint4 (&to)[2 * R][2], int kb) {
+  for (int i = 0; i < 2; ++i) rows[i] = p.w + (long long)min(n0 + g + 8 * i, p.N - 1) * p.ldw + 16 * t;
+  uint4 w[2][2][2];
+  const auto ask = [&](uint4 (&to)[2][2], int kb) {
     const int k = kb * GROUP;
     if (k + GROUP <= p.K) {
 #pragma unroll
-      for (int i = 0; i < 2 * R; ++i) {
+      for (int i = 0; i < 2; ++i) {
         to[i][0] = stream_codes(rows[i] + k);
         to[i][1] = stream_codes(rows[i] + k + 64);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 2 * R; ++i) {
+      for (int i = 0; i < 2; ++i) {
         to[i][0] = codes_to_the_end(rows[i] - 16 * t, k + 16 * t, p.K);
         to[i][1] = codes_to_the_end(rows[i] - 16 * t, k + 16 * t + 64, p.K);
       }
     }
   };
   // x and the scales of a block: behind the kernel ahead's, so apart from the weight
-  const float* sw = p.sw + (long long)(min(n0, p.N - 1) / GROUP) * k_blocks;      // 16 R rows lie in one block of scales
+  const float* sw = p.sw + (long long)(min(n0, p.N - 1) / GROUP) * k_blocks;      // 16 rows lie in one block of scales
   const uint8_t* x_row = p.x + min(g, p.M - 1) * p.ldx + 16 * t;
   const uint8_t* x_row8 = NT == 1 ? nullptr : p.x + min(8 + g, p.M - 1) * p.ldx + 16 * t;
   const float* sx = p.sx + min(2 * t, p.M - 1) * p.sx_row;                        // rows of x beyond the last make results that nobody reads
@@ -686,48 +933,38 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params 
     if constexpr (RAW) ask_raw(raw[0], fs[0][2 * NT], kb0);
     else ask_x(xs[0], fs[0], kb0);
   }
-  float acc[R][NT][4];
+  float acc[NT][4];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+
+  const auto add = [&](const uint4 (&from)[2][2], const uint4 (&x)[NT][2], const float (&f)[2 * NT + 1]) {
+    float in[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[r][i][j] = 0.f;
-
-  const auto add = [&](const uint4 (&from)[2 * R][2], const uint4 (&x)[NT][2], const float (&f)[2 * NT + 1]) {
-    float in[R][NT][4];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) in[r][i][j] = 0.f;
+      for (int j = 0; j < 4; ++j) in[i][j] = 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint32_t b[NT][2];
+        uint32_t a0, a1, a2, a3, b0, b1;
+        halves(word_of(from[0][c], j), a0, a2);
+        halves(word_of(from[1][c], j), a1, a3);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) halves(j == 0 ? x[i][c].x : j == 1 ? x[i][c].y : j == 2 ? x[i][c].z : x[i][c].w, b[i][0], b[i][1]);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const uint4 &lo = from[2 * r][c], &hi = from[2 * r + 1][c];
-          uint32_t a0, a1, a2, a3;
-          halves(j == 0 ? lo.x : j == 1 ? lo.y : j == 2 ? lo.z : lo.w, a0, a2);
-          halves(j == 0 ? hi.x : j == 1 ? hi.y : j == 2 ? hi.z : hi.w, a1, a3);
-#pragma unroll
-          for (int i = 0; i < NT; ++i) mma_16x8x16(in[r][i], a0, a1, a2, a3, b[i][0], b[i][1]);
+        for (int i = 0; i < NT; ++i) {
+          halves(word_of(x[i][c], j), b0, b1);
+          mma_16x8x16(in[i], a0, a1, a2, a3, b0, b1);
         }
       }
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[r][i][j] = fmaf(in[r][i][j], f[2 * i + (j & 1)] * f[2 * NT], acc[r][i][j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(in[i][j], f[2 * i + (j & 1)] * f[2 * NT], acc[i][j]);
   };
   if constexpr (RAW) {
-    const auto add_raw = [&](const uint4 (&from)[2 * R][2], const RawRow& r, float fw) {
+    const auto add_raw = [&](const uint4 (&from)[2][2], const RawRow& r, float fw) {
       uint4 x[1][2];
       float f[3], scale;
       quantize_row(r, x[0], scale);
@@ -755,37 +992,32 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params 
     }
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sums[warp][16 * r + g + 8 * (j >> 1)][8 * i + 2 * t + (j & 1)] = acc[r][i][j];
+    for (int j = 0; j < 4; ++j) sums[warp][g + 8 * (j >> 1)][8 * i + 2 * t + (j & 1)] = acc[i][j];
   __syncthreads();
-  const int high = groups * 16 * R;
+  const int high = groups * 16;
   for (int i = threadIdx.x; i < high * p.M; i += FEW_THREADS) {
     const int r = i % high, m = i / high, n = blockIdx.x * high + r;
     if (n >= p.N) continue;
     float s = 0.f;
-    for (int q = 0; q < ks; ++q) s += sums[r / (16 * R) * ks + q][r % (16 * R)][m];
+    for (int q = 0; q < ks; ++q) s += sums[(r >> 4) * ks + q][r & 15][m];
     if (p.y_bf16) ((bf16*)p.y)[m * p.ldy + n] = __float2bfloat16_rn(s);
     else ((float*)p.y)[m * p.ldy + n] = s;
   }
 }
 
-template <int NT, int R, bool RAW>
+template <int NT, bool RAW>
 int launch_few_rows(const Fp8Params& p, int sms, cudaStream_t stream) {
-  const int groups = (p.N + 16 * R - 1) / (16 * R), k_blocks = (p.K + GROUP - 1) / GROUP;
+  const int groups = (p.N + 15) / 16, k_blocks = (p.K + GROUP - 1) / GROUP;
   int ks = 1;
   while (ks < 8 && (long long)groups * ks < 8LL * sms && 2 * ks <= k_blocks) ks *= 2;
   const int per = FEW_WARPS / ks, grid = (groups + per - 1) / per;
-  return launch_k(gemm_fp8_few_kernel<NT, R, RAW>, grid, FEW_THREADS, 0, stream, p, ks);
+  return launch_k(gemm_fp8_few_kernel<NT, RAW>, grid, FEW_THREADS, 0, stream, p, ks);
 }
-// whether the product of few rows in bfloat16 quantises them itself
-bool few_takes_raw(int M, int N, int sms) { return M <= 8 && N < 32 * sms; }
 int launch_few(const Fp8Params& p, int sms, cudaStream_t stream) {
-  if (p.raw) return launch_few_rows<1, 1, true>(p, sms, stream);
-  if (p.M > 8) return launch_few_rows<2, 1, false>(p, sms, stream);
-  return p.N >= 32 * sms ? launch_few_rows<1, 2, false>(p, sms, stream) : launch_few_rows<1, 1, false>(p, sms, stream);
+  if (p.raw) return launch_few_rows<1, true>(p, sms, stream);
+  return p.M <= 8 ? launch_few_rows<1, false>(p, sms, stream) : launch_few_rows<2, false>(p, sms, stream);
 }
 
 }  // namespace
@@ -794,16 +1026,16 @@ int launch_few(const Fp8Params& p, int sms, cudaStream_t stream) {
 extern "C" int ie_fp8_quantize_rows(const void* x, int dtype, void* codes, float* scales, int rows, int cols, long long ldx,
                                     long long ldc, long long s_row, long long s_col, cudaStream_t stream);
 
-// bytes of scratch that the product of unquantised rows takes: their codes, then their scales [K / 128][M]
-extern "C" long long ie_gemm_fp8_scratch(int x_dtype, int M, int N, int K) {
-  if (M <= 0 || K <= 0 || x_dtype == IE_E4M3 || (x_dtype == IE_BF16 && few_takes_raw(M, N, device_sms()))) return 0;
+// bytes of scratch that the product of unquantised rows takes, unless it quantises them itself: their codes, then their scales [K / 128][M]
+extern "C" long long ie_gemm_fp8_scratch(int M, int K) {
+  if (M <= 0 || K <= 0) return 0;
   return (long long)M * ((K + 15) / 16 * 16) + 4LL * M * ((K + GROUP - 1) / GROUP);
 }
 
 // x: codes (x_dtype IE_E4M3, with sx) or float32 / bfloat16 rows, which are quantised into scratch first
 extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const void* w, const float* sw, void* y, int y_dtype, int M,
                            int N, int K, long long ldx, long long sx_row, long long sx_col, long long ldw, long long ldy,
-                           void* scratch, cudaStream_t stream) {
+                           void* scratch, long long scratch_bytes, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return IE_OK;
   if (K <= 0) return IE_BAD_SIZE;
   if (y_dtype != IE_F32 && y_dtype != IE_BF16) return IE_BAD_DTYPE;
@@ -816,13 +1048,16 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
   p.split = 1;
   p.early = 0;
   p.raw = nullptr;
-  if (x_dtype == IE_BF16 && few_takes_raw(M, N, sms)) {
+  // Up to 8 rows of a small weight: the kernel saved counts for more than quantising them in every block does (8 x 4096 x 2048: 4.4 us
+  // either way, and half of the host's time; 8 x 2048 x 4096: 7.0 against 5.4, 8 x 8192 x 2048: 7.4 against 6.4)
+  if (x_dtype == IE_BF16 && M <= 8 && N < 32 * sms && K <= 2048) {
     p.raw = x; p.raw_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     p.x = nullptr; p.sx = nullptr; p.ldx = ldx; p.sx_row = p.sx_col = 0;
     return launch_few(p, sms, stream);
   }
   if (x_dtype != IE_E4M3) {
-    if (scratch == nullptr || ((uintptr_t)scratch & 15)) return IE_BAD_ALIGN;
+    if (scratch == nullptr || scratch_bytes < ie_gemm_fp8_scratch(M, K)) return IE_NEEDS_SCRATCH;
+    if ((uintptr_t)scratch & 15) return IE_BAD_ALIGN;
     const long long pitch = (K + 15) / 16 * 16;
     float* scales = reinterpret_cast<float*>((char*)scratch + M * pitch);
     const int rc = ie_fp8_quantize_rows(x, x_dtype, scratch, scales, M, K, ldx, pitch, 1, M, stream);
@@ -832,16 +1067,18 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
   }
   if (((uintptr_t)x & 15) || ldx % 16) return IE_BAD_ALIGN;
   p.x = (const uint8_t*)x; p.sx = sx; p.ldx = ldx; p.sx_row = sx_row; p.sx_col = sx_col;
-  if (M <= 16) return launch_few(p, sms, stream);
+  // A weight of 24 million codes and more pays for the start of the tensor cores' kernel (6 x 128256 x 2048: 47.7 us against 52.4, 16 x
+  // 16384 x 2048: 9.4 against 12.6, but 8 x 8192 x 2048: 7.3 against 6.6, 1 x 2048 x 2048: 5.1 against 3.8)
+  if (M <= 16) return (long long)N * K >= (24LL << 20) ? launch_thin<16>(p, sms, stream) : launch_few(p, sms, stream);
+  // 32 rows: 32 x 2048 x 8192 9.4 us against 10.7 of the tiles below, 32 x 16384 x 2048 11.3 against 12.6 (at 64 rows 14.1 against 11.7)
+  if (M <= 32) return launch_thin<32>(p, sms, stream);
   const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
   // More tiles of 128 x 128 than SMs: pairs take less per result (512 x 8192 x 2048, 256 tiles: 15.8 us against 20.8; at 200 x 2048 x
   // 2048, 32 tiles, 13.4 against 9.3).
   if (M > 128 && tiles > sms) return launch_tiles<true, false>(p, sms, stream);
-  const int k_blocks = (K + GROUP - 1) / GROUP;
-  // As many blocks as can share a tile with all tiles under way at once and 4 blocks of K each: 77 x 2048 x 8192 takes 26.6 us
-  // unsplit, 10.9 by four, 10.0 by six (22 clusters fit, 16 tiles), 16.7 by eight (15 fit: two rounds).
-  for (int s = 2; s <= 8 && 4 * s <= k_blocks; ++s)
-    if (clusters_that_fit(s) >= tiles) p.split = s;
+  // 77 x 2048 x 8192 takes 26.6 us unsplit, 10.9 by four, 10.0 by six (22 clusters fit, 16 tiles), 16.7 by eight (15 fit: two rounds)
+  static FitTable fits;
+  p.split = blocks_a_tile(gemm_fp8_tile_kernel<false, true>, TILE_THREADS, (int)TILE_SMEM, tiles, (K + GROUP - 1) / GROUP, 4, fits);
   return p.split > 1 ? launch_tiles<false, true>(p, sms, stream) : launch_tiles<false, false>(p, sms, stream);
 }
 

@@ -1208,7 +1208,8 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, slots: torch.Tensor |
         _refuse(what, "rows overlap")
     at, to = logits.data_ptr(), out.data_ptr()
     same = at == to and code == IE_F32 and (n < 2 or ld_in == ld_out)
-    if not same and _overlap(logits, out):
+    if (not same and n and at < to + 4 * ((n - 1) * ld_out + vocab) and to < at + (4 if code == IE_F32 else 2) * ((n - 1) * ld_in + vocab)
+            and _overlap(logits, out)):
         _refuse(what, "out shares memory with logits without being logits")
     dev = _here(logits)
     if out.get_device() != dev:
@@ -1820,6 +1821,7 @@ _fa5_lib = None
 FP8 = torch.float8_e4m3fn
 FP8_GROUP = 128          # columns (of a weight: rows too) that share a scale
 IE_E4M3 = 2
+_NEEDS_SCRATCH = -5
 _fp8_lib = None
 
 
@@ -1830,8 +1832,8 @@ def fp8_library():
         P, I, L = c_void_p, c_int, c_longlong
         lib.ie_fp8_quantize_rows.argtypes = [P, I, P, P, I, I, L, L, L, L, P]
         lib.ie_fp8_quantize_blocks.argtypes = [P, I, P, P, I, I, L, L, P]
-        lib.ie_gemm_fp8.argtypes = [P, I, P, P, P, P, I, I, I, I, L, L, L, L, L, P, P]
-        lib.ie_gemm_fp8_scratch.argtypes = [I, I, I, I]
+        lib.ie_gemm_fp8.argtypes = [P, I, P, P, P, P, I, I, I, I, L, L, L, L, L, P, L, P]
+        lib.ie_gemm_fp8_scratch.argtypes = [I, I]
         for name in ("ie_fp8_quantize_rows", "ie_fp8_quantize_blocks", "ie_gemm_fp8"):
             getattr(lib, name).restype = c_int
         lib.ie_gemm_fp8_scratch.restype = c_longlong
@@ -1906,11 +1908,9 @@ def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
                                                 _stream()), what)
 
 
-def gemm_fp8_scratch_bytes(x: torch.Tensor, n: int) -> int:
-    """Bytes that ``gemm_fp8`` needs for the codes of rows ``x`` that it quantises, with a weight of ``n`` rows (0: none)."""
-    if x.dtype is FP8:
-        return 0
-    return int(fp8_library().ie_gemm_fp8_scratch(_CODES[x.dtype], x.shape[0], n, x.shape[1]))
+def gemm_fp8_scratch_bytes(x: torch.Tensor) -> int:
+    """Bytes that hold the codes and scales of rows ``x`` for a ``gemm_fp8`` that quantises them."""
+    return 0 if x.dtype is FP8 else int(fp8_library().ie_gemm_fp8_scratch(x.shape[0], x.shape[1]))
 
 
 def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, x_scales: torch.Tensor | None = None,
@@ -1919,7 +1919,7 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
     [ceil(n / 128), ceil(k / 128)], any positive numbers); ``x`` codes with ``x_scales`` (float32 [m, ceil(k / 128)], any strides), or
     float32 / bfloat16 rows, which are quantised as ``fp8_quantize_rows`` does.  Codes lie as ``fp8_empty`` lays them out.  Sums are
     float32: inside a block of 128 columns on the tensor cores, over the scaled blocks in registers.  ``out`` shares no memory with
-    the operands.  ``scratch`` (uint8, at least ``gemm_fp8_scratch_bytes(x, n)``) takes the codes of rows that are quantised here;
+    the operands.  ``scratch`` (uint8, at least ``gemm_fp8_scratch_bytes(x)``) takes the codes of rows that are quantised here;
     without it they go into memory of this call's own."""
     what = "gemm_fp8"
     n, k, w_pitch = _codes(what, "w", w)
@@ -1954,16 +1954,24 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
     if m == 0 or n == 0:
         return
     lib = fp8_library()
-    need = lib.ie_gemm_fp8_scratch(code, m, n, k) if code != IE_E4M3 else 0
-    if not need:
-        scratch = None
-    elif scratch is None:
-        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
-    elif (scratch.dtype is not torch.uint8 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16
-          or scratch.get_device() != dev):
-        _refuse(what, f"scratch is {need} contiguous bytes that start on 16, beside the operands")
-    _check(lib.ie_gemm_fp8(x.data_ptr(), code, scales, w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), to, m, n, k, ldx, s_row, s_col,
-                           w_pitch, ldy, None if scratch is None else scratch.data_ptr(), _stream()), what)
+    y, stream = out.data_ptr(), _stream()
+    args = (x.data_ptr(), code, scales, w.data_ptr(), w_scales.data_ptr(), y, to, m, n, k, ldx, s_row, s_col, w_pitch, ldy)
+    room, size = None, 0
+    if scratch is not None:
+        size = scratch.numel()
+        if scratch.dtype is not torch.uint8 or not scratch.is_contiguous() or scratch.data_ptr() % 16 or scratch.get_device() != dev:
+            _refuse(what, "scratch is contiguous bytes that start on 16, beside the operands")
+        room = scratch.data_ptr()
+    elif code != IE_E4M3 and (m > 8 or code == IE_F32):                # few bfloat16 rows may need none: the call says so
+        own = x.new_empty(gemm_fp8_scratch_bytes(x), dtype=torch.uint8)
+        room, size = own.data_ptr(), own.numel()
+    rc = lib.ie_gemm_fp8(*args, room, size, stream)
+    if rc == _NEEDS_SCRATCH:
+        if scratch is not None:
+            _refuse(what, f"scratch holds {size} bytes, the rows' codes take {gemm_fp8_scratch_bytes(x)}")
+        own = x.new_empty(gemm_fp8_scratch_bytes(x), dtype=torch.uint8)
+        rc = lib.ie_gemm_fp8(*args, own.data_ptr(), own.numel(), stream)
+    _check(rc, what)
 
 
 def attention_tcgen05_library():

@@ -90,8 +90,8 @@ class Linear:
         if x.shape[0] == 0:
             return out
         if self.scales is not None:
-            n = kernels.gemm_fp8_scratch_bytes(x, self.out_features)
-            kernels.gemm_fp8(x, w, self.scales, out, scratch=self.rt.ws.take("fp8_rows", (n,), torch.uint8) if n else None)
+            kernels.gemm_fp8(x, w, self.scales, out,
+                             scratch=self.rt.ws.take("fp8_rows", (kernels.gemm_fp8_scratch_bytes(x),), torch.uint8))
             return out
         if x.dtype is torch.float32 or w.dtype is torch.float32:
             kernels.gemm_simt(x, w, out)

@@ -123,7 +123,8 @@ def test_rows_of_other_strides():
 
 SHAPES = [(1, 128, 128), (1, 1, 1), (1, 16, 16), (2, 130, 100), (7, 2048, 2048), (8, 100, 127), (9, 257, 129), (16, 640, 1000),
           (17, 2050, 2048), (31, 300, 4100), (33, 128, 64), (64, 2048, 512), (65, 129, 8192), (100, 1000, 144), (128, 256, 256),
-          (129, 257, 384), (200, 2048, 2048), (300, 511, 1030), (520, 768, 640), (1, 40000, 256), (16, 128, 16384), (1000, 24, 256)]
+          (129, 257, 384), (200, 2048, 2048), (300, 511, 1030), (520, 768, 640), (1, 40000, 256), (16, 128, 16384), (1000, 24, 256),
+          (1, 25000, 1010), (5, 40000, 700), (13, 3001, 8400), (16, 130, 200000), (2, 12700, 2048), (32, 300, 1000), (24, 20000, 130), (9, 6144, 4097)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
