@@ -308,9 +308,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
     const int quarter = warp & 3, half = (warp - 4) >> 2;          // tensor memory lanes 32 quarter .., columns COLS half ..
     const uint32_t my_tmem = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * COLS);
     const uint32_t first_empty = PAIR ? map_shared(acc_empty0, 0) : acc_empty0;
-    // The scales of a block come AHEAD blocks early into a slot of each thread's own (a load of theirs takes as long as several
-    // blocks' MMAs), on into the next tile.
-    const uint32_t slots = ring + STAGES * STAGE + 8 * OUT_STAGE + (tid - 128) * 8;
+    // The scales of a block come AHEAD blocks early into slots of the warp's own (a load of theirs takes as long as several blocks' MMAs),
+    // on into the next tile: 32 of x side by side, then the one of w, copied once.  (Shared memory feeds the MMAs too: with a
+    // copy of w's scale for every lane, 8 bytes apart, the copies took 300 of its cycles a block.)
+    constexpr uint32_t SLOT = 36 * 4;
+    const uint32_t slots = ring + STAGES * STAGE + 8 * OUT_STAGE + (warp - 4) * AHEAD * SLOT;
     int ahead_t = t0, ahead_kb = kb0, ahead_slot = 0;
     const float *ahead_sx = nullptr, *ahead_sw = nullptr;
     const auto ask = [&]() {
@@ -320,9 +322,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
           ahead_sx = p.sx + min(m, p.M - 1) * p.sx_row + kb0 * p.sx_col;
           ahead_sw = p.sw + (long long)(min(n, p.N - 1) / GROUP) * k_blocks + kb0;
         }
-        const uint32_t dst = slots + ahead_slot * 256 * 8;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(ahead_sx) : "memory");
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4), "l"(ahead_sw) : "memory");
+        const uint32_t dst = slots + ahead_slot * SLOT;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * lane), "l"(ahead_sx) : "memory");
+        if (lane == 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 128), "l"(ahead_sw) : "memory");
         ahead_sx += p.sx_col;
         ++ahead_sw;
         if (++ahead_kb == kb1) { ahead_kb = kb0; ahead_t += t_step; }
@@ -342,10 +344,12 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
 #pragma unroll 1
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int buf = it & 1;
-        ask();
+        ask();                                         // into the slot of the block before, which every lane has read
         asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        __syncwarp();                                  // lane 0's copy of w's scale is there for all
         float fx, fw;
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(fx), "=f"(fw) : "r"(slots + (it % AHEAD) * 256 * 8) : "memory");
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(fx) : "r"(slots + (it % AHEAD) * SLOT + 4 * lane) : "memory");
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(fw) : "r"(slots + (it % AHEAD) * SLOT + 128) : "memory");
         const unsigned long long f = pair(fx * fw, fx * fw);
         ok = bar_wait(acc_full0 + 8 * buf, (uint32_t)(it >> 1) & 1u, &failed);
         if (!ok) { atomicExch(&g_fp8_error, 4); failed = 1; }
@@ -692,7 +696,7 @@ int make_map(CUtensorMap* map, const void* base, int rows, int cols, long long l
   return r == CUDA_SUCCESS ? IE_OK : IE_BAD_ALIGN;
 }
 
-constexpr size_t TILE_SMEM = 1024 + STAGES * STAGE + 8 * OUT_STAGE + AHEAD * 256 * 8;
+constexpr size_t TILE_SMEM = 1024 + STAGES * STAGE + 8 * OUT_STAGE + 8 * AHEAD * 36 * 4;
 
 // clusters of `size` blocks of a kernel that the current device runs at once; `known`: what was asked before, by device and size
 typedef std::atomic<int> FitTable[64][9];
