@@ -204,7 +204,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
   constexpr int TM = PAIR ? 256 : 128, TN = PAIR ? 256 : 128;          // the tile
   constexpr int COLS = TN / 2;                                         // columns of a summing warp: of one block of w's scales
 
-  pdl_trigger();
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t ring = (saddr(smem_raw) + 1023u) & ~1023u;
   unsigned char* ring_ptr = smem_raw + (ring - saddr(smem_raw));
@@ -244,6 +243,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
   else __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
+  pdl_trigger();                                       // a kernel that starts beside this one finds tensor memory taken, not this one
   if (warp < 4) {
     if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
     if (warp == 0) {
@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) gemm_fp8_tile_kernel(const __
       }
       if (failed) for (int i = 0; i < 2048; ++i) __nanosleep(64);        // copies under way still land in this block's memory
     } else if (warp == 1 && (rank == 0 || !PAIR)) {
+      pdl_wait();                                      // its waits have a limit: they begin when the kernel ahead is done
       int s = 0, buf = 0;
       uint32_t phase = 0, acc_phase = 1;
       bool ok = true;
@@ -473,7 +474,6 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) gemm_fp8_thin_kernel(const __
   __shared__ volatile int failed;
   static_assert(TX * PITCH * 4 <= NS * BYTES, "the sums of a split tile fit the ring");
 
-  pdl_trigger();
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t ring = (saddr(smem_raw) + 1023u) & ~1023u;
   unsigned char* ring_ptr = smem_raw + (ring - saddr(smem_raw));
@@ -505,6 +505,7 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) gemm_fp8_thin_kernel(const __
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
+  pdl_trigger();                                       // a kernel that starts beside this one finds tensor memory taken, not this one
 
   if (warp == 0) {
     int s = 0;
@@ -537,6 +538,7 @@ __global__ void __launch_bounds__(THIN_THREADS, 1) gemm_fp8_thin_kernel(const __
     }
     if (failed) for (int i = 0; i < 2048; ++i) __nanosleep(64);      // copies under way still land in this block's memory
   } else if (warp == 1) {
+    pdl_wait();                                        // its waits have a limit: they begin when the kernel ahead is done
     int s = 0, buf = 0;
     uint32_t phase = 0, acc_phase = 1;
     bool ok = true;

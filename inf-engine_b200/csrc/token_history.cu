@@ -107,7 +107,7 @@ struct AdjustParams {
 constexpr int ADJUST_STEPS = 4, ADJUST_TOKENS = 4096;
 
 template <typename T, int V>
-__global__ void __launch_bounds__(HT) adjust_logits_kernel(AdjustParams p) {
+__global__ void __launch_bounds__(HT, 8) adjust_logits_kernel(AdjustParams p) {
   __shared__ unsigned short list[ADJUST_TOKENS];       // tokens to penalise, from the block's first on, in no order that matters
   __shared__ int listed;
   pdl_trigger();
@@ -124,9 +124,6 @@ __global__ void __launch_bounds__(HT) adjust_logits_kernel(AdjustParams p) {
   const int* seen = slot >= 0 ? p.seen + (size_t)slot * p.words : nullptr;
   const int* counts = slot >= 0 ? p.counts + (size_t)slot * p.vocab : nullptr;
   const int* mask = mask_row >= 0 ? p.masks + (size_t)mask_row * p.words : nullptr;
-  // the row's biases, and the first of them for each thread, under way before anything waits
-  const int b0 = p.bias_start != nullptr ? max(0, p.bias_start[row]) : 0, b1 = p.bias_start != nullptr ? min(p.n_bias, p.bias_start[row + 1]) : 0;
-  const int first_bias = b0 + (int)threadIdx.x < b1 ? p.bias_ids[b0 + threadIdx.x] : -1;
   if (seen) {
     for (int w = (lo >> 5) + threadIdx.x; w < (hi + 31) >> 5; w += HT) {
       unsigned bits = (unsigned)seen[w] & (mask ? (unsigned)mask[w] : 0xffffffffu);
@@ -188,13 +185,15 @@ __global__ void __launch_bounds__(HT) adjust_logits_kernel(AdjustParams p) {
       out[t] = v;
     }
   }
+  if (p.bias_start == nullptr) return;
+  const int b0 = max(0, p.bias_start[row]), b1 = min(p.n_bias, p.bias_start[row + 1]);
   if (b0 >= b1) return;
   __syncthreads();
   // 32 biases a warp at a time; for each one that falls into this block's logits the whole warp looks through the row's list, for a
   // token that comes twice: its first bias takes all of them, in order, and the later ones nothing
   const int lane = threadIdx.x & 31;
   for (int bw = b0 + (threadIdx.x & ~31); bw < b1; bw += HT) {
-    const int mine = bw < b0 + HT ? first_bias : bw + lane < b1 ? p.bias_ids[bw + lane] : -1;
+    const int mine = bw + lane < b1 ? p.bias_ids[bw + lane] : -1;
     const bool takes = mine >= lo && mine < hi && !(mask && !((mask[mine >> 5] >> (mine & 31)) & 1));
     for (unsigned left = __ballot_sync(0xffffffffu, takes); left; left &= left - 1) {
       const int at = bw + __ffs(left) - 1, t = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);

@@ -149,7 +149,7 @@ class Engine:
         s = self.scheduler
         if self.cfg.windowed:
             return False
-        for r in list(s.running) + s.queue[:4]:
+        for r in list(s.running) + s.queue[:s.max_batch - len(s.running)]:      # those that the plan may admit
             c = r.sampling or self.cfg
             if c.windowed or r.allowed_tokens is not None:
                 return False

@@ -1858,6 +1858,8 @@ def _codes(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
         _refuse(what, f"{name} is a float8_e4m3fn matrix")
     rows, cols = t.shape
     pitch, step = t.stride()
+    if rows < 2:
+        pitch = max(16, -(-cols // 16) * 16)         # one row lies nowhere from the next
     if (step != 1 and cols > 1) or pitch % 16 or pitch < cols or t.data_ptr() % 16:
         _refuse(what, f"rows of {name} are adjacent codes and start on 16 bytes")
     return rows, cols, pitch
@@ -1954,8 +1956,12 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
     if m == 0 or n == 0:
         return
     lib = fp8_library()
-    y, stream = out.data_ptr(), _stream()
-    args = (x.data_ptr(), code, scales, w.data_ptr(), w_scales.data_ptr(), y, to, m, n, k, ldx, s_row, s_col, w_pitch, ldy)
+    at, y, stream = x.data_ptr(), out.data_ptr(), _stream()
+    end = y + (4 if to == IE_F32 else 2) * ((m - 1) * ldy + n)
+    if ((y < at + (1 if code == IE_E4M3 else 2 if code else 4) * ((m - 1) * ldx + k) and at < end and _overlap(x, out))
+            or (y < w.data_ptr() + (n - 1) * w_pitch + k and w.data_ptr() < end and _overlap(w, out))):
+        _refuse(what, "out shares memory with an operand")
+    args = (at, code, scales, w.data_ptr(), w_scales.data_ptr(), y, to, m, n, k, ldx, s_row, s_col, w_pitch, ldy)
     room, size = None, 0
     if scratch is not None:
         size = scratch.numel()

@@ -204,6 +204,53 @@ def test_a_number_that_is_none_stays_in_its_row(m):
     assert torch.equal(out[keep], clean[keep])
 
 
+def test_out_shares_no_memory_with_an_operand():
+    k = 256
+    w, sw = quantized(rows(256, k, torch.bfloat16, 1, wide=False), 128)
+    x = rows(20, k, torch.bfloat16, 2)
+    with pytest.raises(kernels.KernelError, match="shares memory"):
+        kernels.gemm_fp8(x, w, sw, x)
+    with pytest.raises(kernels.KernelError, match="shares memory"):
+        kernels.gemm_fp8(x, w, sw, w.view(torch.bfloat16).view(-1)[:20 * 256].view(20, 256))
+    buf = torch.empty(20, 600, dtype=torch.bfloat16, device="cuda")       # side by side is no overlap
+    buf[:, :k] = x
+    kernels.gemm_fp8(buf[:, :k], w, sw, buf[:, 300:556])
+    want, mag = expect(*quantized(x), w, sw)
+    check_product(buf[:, 300:556], want, mag, k)
+    small = torch.empty(16, dtype=torch.uint8, device="cuda")
+    with pytest.raises(kernels.KernelError, match="scratch holds"):
+        kernels.gemm_fp8(x, w, sw, torch.empty(20, 256, device="cuda"), scratch=small)
+
+
+FIRST = """
+import torch
+from inf_engine_b200 import kernels
+M, N, K = {m}, {n}, {k}
+w = torch.ones(N, K, device="cuda")
+codes, scales = kernels.fp8_empty(N, K, "cuda"), torch.empty(-(-N // 128), -(-K // 128), device="cuda")
+x, out = torch.ones(M, K, device="cuda", dtype=torch.bfloat16), torch.zeros(M, N, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    kernels.fp8_quantize_blocks(w, codes, scales)
+    kernels.gemm_fp8(x, codes, scales, out)
+g.replay()
+torch.cuda.synchronize()
+assert bool((out == K).all())
+assert kernels.gemm_fp8_error() == 0
+"""
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (12, 256, 512), (16, 13000, 2048), (24, 256, 1024), (100, 256, 1024), (300, 5120, 512)])
+def test_the_first_call_of_a_program_may_be_captured(m, n, k):
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FIRST.format(m=m, n=n, k=k)], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0, r.stderr[-1500:]
+
+
 def test_empty_products():
     w, sw = quantized(rows(20, 64, torch.bfloat16), 128)
     kernels.gemm_fp8(torch.empty(0, 64, device="cuda"), w, sw, torch.empty(0, 20, device="cuda"))

@@ -118,6 +118,16 @@ def test_masks(tmp_path):
     check(weights, config, requests, out, lambda r, said: r.allowed_tokens(said) if r.allowed_tokens else None)
 
 
+def test_requests_admitted_together_keep_their_masks(tmp_path):
+    """A mask needs its request's tokens on the host, wherever in the queue it stands when a step admits it."""
+    from inf_engine_b200 import Engine, Request
+    d = make_model_dir(tmp_path, "tiny_a")
+    engine = Engine.from_dir(d, dtype="float32", n_total_blocks=128, block_size=8, max_requests=12)
+    requests = [Request(i, [i + 1, 5], 6, allowed_tokens=(lambda g: [7 + len(g)]) if i == 9 else None) for i in range(11)]
+    out = engine.run_offline(requests)
+    assert out[9] == [7, 8, 9, 10, 11, 12]
+
+
 def test_refused_requests(tmp_path):
     from inf_engine_b200 import Engine, Request, SamplingConfig
     d = make_model_dir(tmp_path, "tiny_a")

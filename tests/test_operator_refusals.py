@@ -59,6 +59,8 @@ def test_product():
     refused("k is 0", g, torch.zeros(3, 0), codes(130, 0), torch.ones(2, 0), out)
     refused("current device", g, x, w, sw, out)
     refused("current device", g, q, w, sw, out, sx)
+    one = torch.zeros(1, 200, dtype=torch.uint8).view(FP8)                # one row needs no room behind it
+    refused("current device", g, one, w, sw, out[:1], sx[:1])
 
 
 def test_history():
