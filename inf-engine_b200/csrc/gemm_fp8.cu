@@ -1033,7 +1033,7 @@ extern "C" int ie_fp8_quantize_rows(const void* x, int dtype, void* codes, float
                                     long long ldc, long long s_row, long long s_col, cudaStream_t stream);
 
 // bytes of scratch that the product of unquantised rows takes, unless it quantises them itself: their codes, then their scales [K / 128][M]
-extern "C" long long ie_gemm_fp8_scratch(int M, int K) {
+static long long scratch_of(int M, int K) {
   if (M <= 0 || K <= 0) return 0;
   return (long long)M * ((K + 15) / 16 * 16) + 4LL * M * ((K + GROUP - 1) / GROUP);
 }
@@ -1062,7 +1062,7 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
     return launch_few(p, sms, stream);
   }
   if (x_dtype != IE_E4M3) {
-    if (scratch == nullptr || scratch_bytes < ie_gemm_fp8_scratch(M, K)) return IE_NEEDS_SCRATCH;
+    if (scratch == nullptr || scratch_bytes < scratch_of(M, K)) return IE_NEEDS_SCRATCH;
     if ((uintptr_t)scratch & 15) return IE_BAD_ALIGN;
     const long long pitch = (K + 15) / 16 * 16;
     float* scales = reinterpret_cast<float*>((char*)scratch + M * pitch);

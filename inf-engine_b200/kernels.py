@@ -1105,6 +1105,7 @@ def _here(t: torch.Tensor) -> int:
     return d if d >= 0 and d == torch._C._cuda_getDevice() else -2
 
 
+_stream_of = torch._C._cuda_getCurrentRawStream      # of a device by its index
 _I32, _F32 = torch.int32, torch.float32
 
 
@@ -1124,9 +1125,10 @@ def history_reset(counts: torch.Tensor, seen: torch.Tensor, slots: torch.Tensor)
     n_slots, vocab = _history("history_reset", counts, seen)
     if slots.dim() != 1 or slots.dtype is not _I32 or not slots.is_contiguous():
         _refuse("history_reset", "slots is a contiguous int32 [n]")
-    if not _here(counts) == seen.get_device() == slots.get_device():
+    dev = _here(counts)
+    if not dev == seen.get_device() == slots.get_device():
         _away("history_reset", counts, seen, slots)
-    _check(core().ie_history_reset(counts.data_ptr(), seen.data_ptr(), slots.data_ptr(), slots.shape[0], n_slots, vocab, _stream()),
+    _check(core().ie_history_reset(counts.data_ptr(), seen.data_ptr(), slots.data_ptr(), slots.shape[0], n_slots, vocab, _stream_of(dev)),
            "history_reset")
 
 
@@ -1162,7 +1164,7 @@ def history_append(counts: torch.Tensor, seen: torch.Tensor, tokens: torch.Tenso
         _away(what, counts, seen, tokens, slots, starts, n_prompt)
     _check(core().ie_history_append(counts.data_ptr(), seen.data_ptr(), tokens.data_ptr(), slots.data_ptr(),
                                     None if starts is None else starts.data_ptr(), None if n_prompt is None else n_prompt.data_ptr(),
-                                    n, r, n_slots, vocab, _stream()), what)
+                                    n, r, n_slots, vocab, _stream_of(dev)), what)
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -1253,7 +1255,7 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, slots: torch.Tensor |
     if dev < 0:
         _away(what, logits, out, slots, penalties, counts, seen, bias_start, bias_ids, bias_values, mask_rows, masks)
     _check(core().ie_adjust_logits(at, code, to, p_slots, p_pen, p_counts, p_seen, p_start, p_ids, p_values, p_rows, p_masks, n, vocab,
-                                   ld_in, ld_out, n_slots, n_bias, n_masks, 1 if same else 0, _stream()), what)
+                                   ld_in, ld_out, n_slots, n_bias, n_masks, 1 if same else 0, _stream_of(dev)), what)
 
 
 # ------------------------------------------------- tensor-core attention (bfloat16)
@@ -1833,10 +1835,8 @@ def fp8_library():
         lib.ie_fp8_quantize_rows.argtypes = [P, I, P, P, I, I, L, L, L, L, P]
         lib.ie_fp8_quantize_blocks.argtypes = [P, I, P, P, I, I, L, L, P]
         lib.ie_gemm_fp8.argtypes = [P, I, P, P, P, P, I, I, I, I, L, L, L, L, L, P, L, P]
-        lib.ie_gemm_fp8_scratch.argtypes = [I, I]
         for name in ("ie_fp8_quantize_rows", "ie_fp8_quantize_blocks", "ie_gemm_fp8"):
             getattr(lib, name).restype = c_int
-        lib.ie_gemm_fp8_scratch.restype = c_longlong
         lib.ie_gemm_fp8_error.restype = c_int
         _fp8_lib = lib
     return _fp8_lib
@@ -1883,15 +1883,16 @@ def fp8_quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
     what = "fp8_quantize_rows"
     code = _rows_in(what, "x", x)
     n, k, pitch = _codes(what, "codes", codes)
-    if x.shape != codes.shape:
+    if x.shape != (n, k):
         _refuse(what, "codes has another shape than x")
     if scales.shape != (n, (k + 127) // 128) or scales.dtype is not _F32:
         _refuse(what, "scales is float32 [n, ceil(k / 128)]")
-    if not _here(x) == codes.get_device() == scales.get_device():
+    dev = _here(x)
+    if not dev == codes.get_device() == scales.get_device():
         _away(what, x, codes, scales)
     s_row, s_col = scales.stride()
     _check(fp8_library().ie_fp8_quantize_rows(x.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), n, k, x.stride(0), pitch, s_row,
-                                              s_col, _stream()), what)
+                                              s_col, _stream_of(dev)), what)
 
 
 def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
@@ -1900,19 +1901,21 @@ def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     what = "fp8_quantize_blocks"
     code = _rows_in(what, "w", w)
     n, k, pitch = _codes(what, "codes", codes)
-    if w.shape != codes.shape:
+    if w.shape != (n, k):
         _refuse(what, "codes has another shape than w")
     if scales.shape != ((n + 127) // 128, (k + 127) // 128) or scales.dtype is not _F32 or not scales.is_contiguous():
         _refuse(what, "scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
-    if not _here(w) == codes.get_device() == scales.get_device():
+    dev = _here(w)
+    if not dev == codes.get_device() == scales.get_device():
         _away(what, w, codes, scales)
     _check(fp8_library().ie_fp8_quantize_blocks(w.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), n, k, w.stride(0), pitch,
-                                                _stream()), what)
+                                                _stream_of(dev)), what)
 
 
 def gemm_fp8_scratch_bytes(x: torch.Tensor) -> int:
     """Bytes that hold the codes and scales of rows ``x`` for a ``gemm_fp8`` that quantises them."""
-    return 0 if x.dtype is FP8 else int(fp8_library().ie_gemm_fp8_scratch(x.shape[0], x.shape[1]))
+    m, k = x.shape
+    return 0 if x.dtype is FP8 else m * ((k + 15) // 16 * 16 + 4 * ((k + 127) // 128))     # checked against in gemm_fp8.cu
 
 
 def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, x_scales: torch.Tensor | None = None,
@@ -1956,7 +1959,7 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
     if m == 0 or n == 0:
         return
     lib = fp8_library()
-    at, y, stream = x.data_ptr(), out.data_ptr(), _stream()
+    at, y, stream = x.data_ptr(), out.data_ptr(), _stream_of(dev)
     end = y + (4 if to == IE_F32 else 2) * ((m - 1) * ldy + n)
     if ((y < at + (1 if code == IE_E4M3 else 2 if code else 4) * ((m - 1) * ldx + k) and at < end and _overlap(x, out))
             or (y < w.data_ptr() + (n - 1) * w_pitch + k and w.data_ptr() < end and _overlap(w, out))):
