@@ -702,9 +702,8 @@ constexpr size_t TILE_SMEM = 1024 + STAGES * STAGE + 8 * OUT_STAGE + 8 * AHEAD *
 
 // clusters of `size` blocks of a kernel that the current device runs at once; `known`: what was asked before, by device and size
 typedef std::atomic<int> FitTable[64][9];
-int clusters_that_fit(const void* kernel, int threads, int smem, int size, FitTable& known) {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+int clusters_that_fit(int dev, const void* kernel, int threads, int smem, int size, FitTable& known) {
+  int n = 0;
   if (dev < 64 && (n = known[dev][size].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
@@ -727,9 +726,10 @@ int clusters_that_fit(const void* kernel, int threads, int smem, int size, FitTa
 // As many blocks as can share a tile with all tiles under way at once and `least` blocks of K each
 template <typename Kernel>
 int blocks_a_tile(Kernel kernel, int threads, int smem, long long tiles, int k_blocks, int least, FitTable& known) {
-  int split = 1;
+  int split = 1, dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return split;
   for (int s = 2; s <= 8 && least * s <= k_blocks; ++s)
-    if (clusters_that_fit((const void*)kernel, threads, smem, s, known) >= tiles) split = s;
+    if (clusters_that_fit(dev, (const void*)kernel, threads, smem, s, known) >= tiles) split = s;
   return split;
 }
 

@@ -1823,6 +1823,8 @@ _fa5_lib = None
 FP8 = torch.float8_e4m3fn
 FP8_GROUP = 128          # columns (of a weight: rows too) that share a scale
 IE_E4M3 = 2
+_OPERANDS = {**_CODES, FP8: IE_E4M3}
+_BYTES = {IE_F32: 4, IE_BF16: 2, IE_E4M3: 1}
 _NEEDS_SCRATCH = -5
 _fp8_lib = None
 
@@ -1928,14 +1930,20 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
     without it they go into memory of this call's own."""
     what = "gemm_fp8"
     n, k, w_pitch = _codes(what, "w", w)
-    if x.dim() != 2 or x.shape[1] != k or out.shape != (x.shape[0], n):
+    code, to = _OPERANDS.get(x.dtype), _CODES.get(out.dtype)
+    if x.dim() != 2 or code is None:
+        _refuse(what, "x is a matrix of float32, bfloat16 or float8_e4m3fn")
+    m, kx = x.shape
+    if kx != k or out.shape != (m, n):
         _refuse(what, "x is [m, k], w [n, k], out [m, n]")
-    m = x.shape[0]
-    to = _CODES.get(out.dtype)
-    ldy = out.stride(0)
-    if to is None or (out.stride(1) != 1 and n > 1) or (m > 1 and ldy < n):
+    ldx, step = x.stride()
+    if step != 1 and k > 1:
+        _refuse(what, "columns of x are adjacent")
+    ldy, step = out.stride()
+    if to is None or (step != 1 and n > 1) or (m > 1 and ldy < n):
         _refuse(what, "out is a float32 or bfloat16 matrix of adjacent columns")
-    if w_scales.shape != ((n + 127) // 128, (k + 127) // 128) or w_scales.dtype is not _F32 or not w_scales.is_contiguous():
+    kb = (k + 127) // 128
+    if w_scales.shape != ((n + 127) // 128, kb) or w_scales.dtype is not _F32 or not w_scales.is_contiguous():
         _refuse(what, "w_scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
     if k == 0:
         _refuse(what, "k is 0")
@@ -1943,28 +1951,27 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
     if not dev == w.get_device() == w_scales.get_device() == out.get_device():
         dev = -2
     scales, s_row, s_col = None, 0, 0
-    if x.dtype is FP8:
-        code, ldx = IE_E4M3, _codes(what, "x", x)[2]
-        if x_scales is None or x_scales.shape != (m, (k + 127) // 128) or x_scales.dtype is not _F32:
+    if code == IE_E4M3:
+        ldx = _codes(what, "x", x)[2]
+        if x_scales is None or x_scales.shape != (m, kb) or x_scales.dtype is not _F32:
             _refuse(what, "codes of x come with x_scales, float32 [m, ceil(k / 128)]")
         if x_scales.get_device() != dev:
             dev = -2
         scales, (s_row, s_col) = x_scales.data_ptr(), x_scales.stride()
-    else:
-        code, ldx = _rows_in(what, "x", x), x.stride(0)
-        if x_scales is not None:
-            _refuse(what, "x_scales go with codes of x")
+    elif x_scales is not None:
+        _refuse(what, "x_scales go with codes of x")
     if dev < 0:
         _away(what, x, w, w_scales, out, x_scales)
     if m == 0 or n == 0:
         return
     lib = fp8_library()
-    at, y, stream = x.data_ptr(), out.data_ptr(), _stream_of(dev)
-    end = y + (4 if to == IE_F32 else 2) * ((m - 1) * ldy + n)
-    if ((y < at + (1 if code == IE_E4M3 else 2 if code else 4) * ((m - 1) * ldx + k) and at < end and _overlap(x, out))
-            or (y < w.data_ptr() + (n - 1) * w_pitch + k and w.data_ptr() < end and _overlap(w, out))):
+    at, of, y = x.data_ptr(), w.data_ptr(), out.data_ptr()
+    end = y + _BYTES[to] * ((m - 1) * ldy + n)
+    if ((y < at + _BYTES[code] * ((m - 1) * ldx + k) and at < end and _overlap(x, out))
+            or (y < of + (n - 1) * w_pitch + k and of < end and _overlap(w, out))):
         _refuse(what, "out shares memory with an operand")
-    args = (at, code, scales, w.data_ptr(), w_scales.data_ptr(), y, to, m, n, k, ldx, s_row, s_col, w_pitch, ldy)
+    args = (at, code, scales, of, w_scales.data_ptr(), y, to, m, n, k, ldx, s_row, s_col, w_pitch, ldy)
+    stream = _stream_of(dev)
     room, size = None, 0
     if scratch is not None:
         size = scratch.numel()
