@@ -9,7 +9,9 @@
 // relative: 2^-4), whichever way the quotient is computed.  A largest / 448 that is no power of two would gain nothing but
 // the last binade's top (448 is used to between 0.5 and 1) and cost a second rounding.
 //
-// Both read every number once and write a byte for it; the HBM rate is the bound.
+// Both read every number once and write a byte for it; the HBM rate is the bound: 4,096 rows of 8,192 in bfloat16 take 18.4 us (5.5
+// TB/s), in float32 25.7 (6.5), a weight of 16,384 x 2,048 in bfloat16 19.1 us (5.3).  With a look at every number for infinities
+// (now only where a group's largest is one) and 8 numbers a lane the bfloat16 rows took 28 us: instructions.
 #include "fp8_codes.cuh"
 
 namespace {

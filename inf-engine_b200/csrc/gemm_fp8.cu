@@ -4,6 +4,14 @@
 //   y[m, n] = sum_b sx[m, b] sw[n / 128, b]  sum_{k in block b} x[m, k] w[n, k]
 //
 // inner and outer sums in float32, one rounding to the output's type.
+//
+// Four kernels, by the rows of x and the length of the weight (ie_gemm_fp8 holds the rules, with both sides measured):
+//   few rows          registers and the matrix instructions for halves; bfloat16 rows may be quantised inside
+//   a long weight     under up to 32 rows: the tensor cores, w as the larger operand, bound by the weight's bytes (5.6 TB/s)
+//   tiles             128 x 128, K dealt out over a cluster where tiles are few
+//   pairs             256 x 256 over two SMs: 4096 x 8192 x 8192 in 237 us (2.32 PFLOP/s; 276 us and 1.99 under the card's power
+//                     cap).  The library's product of the same codes with one scale for all takes 190 and 220: the rest is the
+//                     scaling of every block of 128, 2.1 thousand million multiply-adds out of tensor memory.
 #include "fp8_codes.cuh"
 #include <cooperative_groups.h>
 #include <cuda.h>

@@ -11,6 +11,10 @@
 //   v += the row's biases for t;   a row with a mask:  v = -inf where t is not allowed, whatever it was (NaN too)
 // Float32 throughout.  The bits say where counts have to be read at all: a vocabulary of 128,256 has 16 KB of them where the
 // counts are 513 KB, so what a row reads beside its logits is 1/32 of them and a sector for every token it has said.
+//
+// Measured (device): 64 tokens appended 1.9 us, a launch and three dependent loads; 64 slots of 128,256 cleared 6.6 us (5.3 TB/s of
+// stores) and 196,000 tokens added to them 4.9 us; 64 rows of 128,256 logits adjusted 17.9 us with 8,000 tokens seen, 100 biases and
+// a mask on every second row, 11.5 as a copy (5.7 TB/s).
 #include "common.cuh"
 
 namespace {
