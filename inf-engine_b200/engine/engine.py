@@ -157,6 +157,16 @@ class Engine:
                 return False
         return s.cache.n_free_pages() >= len(s.running) + 1
 
+    def _plan(self):
+        plan = self.scheduler.plan()
+        self.stats["preemptions"] += len(plan.preempted)
+        if self.adjuster.history is not None:
+            for r in plan.admitted:
+                slot = self.runner.cache.slots.get(r.req_id)
+                if slot is not None:
+                    self.adjuster.history.forget(slot)
+        return plan
+
     def _history_is_current(self, r: Request) -> bool:
         slot = self.runner.cache.slots.get(r.req_id)
         return slot is not None and self.adjuster.history is not None and self.adjuster.history.current(slot, r)
@@ -185,8 +195,7 @@ class Engine:
     def _step_ahead(self, now: float) -> list[Request]:
         t_host0 = time.perf_counter()
         prev = self._pending
-        plan = self.scheduler.plan()
-        self.stats["preemptions"] += len(plan.preempted)
+        plan = self._plan()
         if not plan.entries:
             return self._drain(now)
         prev_index = {e.request.req_id: i for i, e in enumerate(prev["wanted"])} if prev else {}
@@ -229,8 +238,7 @@ class Engine:
 
     def _step_now(self, now: float) -> list[Request]:
         t_host0 = time.perf_counter()
-        plan = self.scheduler.plan()
-        self.stats["preemptions"] += len(plan.preempted)
+        plan = self._plan()
         if not plan.entries:
             return []
         entries = [StepEntry(e.request.req_id, e.tokens, [len(e.tokens) - 1] if e.wants_logits else [])

@@ -48,6 +48,10 @@ class TokenHistory:
         held = self._holds.get(slot)
         return held is not None and held[0] is request and held[1] == len(request.generated)
 
+    def forget(self, slot: int) -> None:
+        """The slot has got a request, perhaps the one that it had before: nothing is known of what it holds."""
+        self._holds.pop(slot, None)
+
     def enter(self, entries: list[tuple[int, object]]) -> None:
         """Writes the histories of requests anew, from their prompts and generated tokens: ``entries`` are (slot, request)."""
         tokens, starts = [], [0]

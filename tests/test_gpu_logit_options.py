@@ -118,6 +118,19 @@ def test_masks(tmp_path):
     check(weights, config, requests, out, lambda r, said: r.allowed_tokens(said) if r.allowed_tokens else None)
 
 
+def test_a_request_submitted_again_has_a_new_history(tmp_path):
+    from inf_engine_b200 import Engine, Request, SamplingConfig
+    d = make_model_dir(tmp_path, "tiny_a")
+    config, weights = plain_inputs(d)
+    engine = Engine.from_dir(d, dtype="float32", n_total_blocks=64, block_size=8, max_requests=1)
+    r = Request(0, random_tokens(256, 9, 1), 8, sampling=SamplingConfig(repetition_penalty=1.5, repetition_scope="history", frequency_penalty=0.5))
+    for seed in (1, 2, 3):
+        r.prompt_ids, r.generated, r.start_time, r.finish_time = random_tokens(256, 9, seed), [], 0.0, 0.0
+        out = engine.run_offline([r])
+        check(weights, config, [r], out)
+        engine.scheduler.completed.clear()
+
+
 def test_requests_admitted_together_keep_their_masks(tmp_path):
     """A mask needs its request's tokens on the host, wherever in the queue it stands when a step admits it."""
     from inf_engine_b200 import Engine, Request
