@@ -798,9 +798,8 @@ int launch_thin(Fp8Params p, int sms, cudaStream_t stream) {
 // same conversions, of both operands every time; they are what bounds this kernel, so slots in shared memory with more blocks of K
 // ahead do not help: 4 x 8192 x 8192 took 22 us with four, 15.9 so).  The instruction wants of lane (g, t) two numbers from 2 t and two
 // from 8 + 2 t of its 16; any other dealing of K serves as well if both operands share it, so lane t takes 16 neighbouring codes of 64,
-// for four instructions.  ks warps share rows of w and deal out K where there are few rows; their sums come together in shared
+// for four instructions.  ks warps share rows of w and deal out K where there are few rows of it; their sums come together in shared
 // memory, in the order of K.
-constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32;
 
 // 16 codes from column k on, zeros behind the last column (what lies there may be anything, NaN too)
 __device__ __forceinline__ uint4 codes_to_the_end(const uint8_t* row, int k, int K) {
@@ -880,12 +879,12 @@ __device__ __forceinline__ void quantize_row(const RawRow& r, uint4 (&codes)[2],
 }
 
 // RAW: x comes in bfloat16 and is quantised here (one tile of 8 rows)
-template <int NT, bool RAW>
-__global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params p, int ks) {
+template <int NT, bool RAW, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) gemm_fp8_few_kernel(Fp8Params p, int ks) {
   static_assert(!RAW || NT == 1, "registers for one tile of raw rows");
-  __shared__ float sums[FEW_WARPS][16][8 * NT + 1];
+  __shared__ float sums[WARPS][16][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int groups = FEW_WARPS / ks, slice = warp % ks, k_blocks = (p.K + GROUP - 1) / GROUP;
+  const int groups = WARPS / ks, slice = warp % ks, k_blocks = (p.K + GROUP - 1) / GROUP;
   const int n0 = (blockIdx.x * groups + warp / ks) * 16;
   const int kb0 = k_blocks * slice / ks, kb1 = n0 < p.N ? k_blocks * (slice + 1) / ks : kb0;
   const uint8_t* rows[2];
@@ -1011,7 +1010,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params 
     for (int j = 0; j < 4; ++j) sums[warp][g + 8 * (j >> 1)][8 * i + 2 * t + (j & 1)] = acc[i][j];
   __syncthreads();
   const int high = groups * 16;
-  for (int i = threadIdx.x; i < high * p.M; i += FEW_THREADS) {
+  for (int i = threadIdx.x; i < high * p.M; i += 32 * WARPS) {
     const int r = i % high, m = i / high, n = blockIdx.x * high + r;
     if (n >= p.N) continue;
     float s = 0.f;
@@ -1024,10 +1023,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) gemm_fp8_few_kernel(Fp8Params 
 template <int NT, bool RAW>
 int launch_few_rows(const Fp8Params& p, int sms, cudaStream_t stream) {
   const int groups = (p.N + 15) / 16, k_blocks = (p.K + GROUP - 1) / GROUP;
+  // No more row tiles than SMs, and 16 blocks of K: one tile a block of 16 warps, each with a sixteenth of K (against 8 warps 1 x 2048 x 2048
+  // 2.9 us and 4.0, 8 x 2048 x 8192 6.8 and 7.9)
+  if (groups <= sms && k_blocks >= 16) return launch_k(gemm_fp8_few_kernel<NT, RAW, 16>, groups, 512, 0, stream, p, 16);
   int ks = 1;
   while (ks < 8 && (long long)groups * ks < 8LL * sms && 2 * ks <= k_blocks) ks *= 2;
-  const int per = FEW_WARPS / ks, grid = (groups + per - 1) / per;
-  return launch_k(gemm_fp8_few_kernel<NT, RAW>, grid, FEW_THREADS, 0, stream, p, ks);
+  const int per = 8 / ks, grid = (groups + per - 1) / per;
+  return launch_k(gemm_fp8_few_kernel<NT, RAW, 8>, grid, 256, 0, stream, p, ks);
 }
 int launch_few(const Fp8Params& p, int sms, cudaStream_t stream) {
   if (p.raw) return launch_few_rows<1, true>(p, sms, stream);
@@ -1062,9 +1064,10 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
   p.split = 1;
   p.early = 0;
   p.raw = nullptr;
-  // Up to 8 rows of a small weight: the kernel saved counts for more than quantising them in every block does (8 x 4096 x 2048: 4.4 us
-  // either way, and half of the host's time; 8 x 2048 x 4096: 7.0 against 5.4, 8 x 8192 x 2048: 7.4 against 6.4)
-  if (x_dtype == IE_BF16 && M <= 8 && N < 32 * sms && K <= 2048) {
+  // Up to 8 rows of a small weight: the kernel saved counts for more than quantising them in every block does, as long as a warp has two
+  // blocks of K at most (8 x 4096 x 2048: 4.4 us either way, 8 x 2048 x 4096 4.4 against 4.5, and half of the host's time; 8 x 2048 x 8192
+  // 7.7 against 6.8, 8 x 8192 x 2048 7.4 against 6.4)
+  if (x_dtype == IE_BF16 && M <= 8 && N < 32 * sms && K <= (N <= 16 * sms ? 4096 : 2048)) {
     p.raw = x; p.raw_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     p.x = nullptr; p.sx = nullptr; p.ldx = ldx; p.sx_row = p.sx_col = 0;
     return launch_few(p, sms, stream);

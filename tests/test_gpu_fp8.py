@@ -204,6 +204,35 @@ def test_a_number_that_is_none_stays_in_its_row(m):
     assert torch.equal(out[keep], clean[keep])
 
 
+def test_offsets_beyond_32_bits():
+    """A weight and rows of more than 2^32 codes: the last rows are what they are alone."""
+    n, k = 540_000, 8192
+    w = torch.zeros(n, k, dtype=torch.uint8, device="cuda").view(FP8)
+    sw = torch.ones(-(-n // 128), 64, device="cuda")
+    tail, st = quantized(rows(300, k, torch.bfloat16, 1, wide=False), 128)
+    first = n - 300 - (n - 300) % 128                                     # a block of scales starts there
+    w[first:first + 300].copy_(tail)
+    sw[first // 128:first // 128 + 3] = st
+    for m in (3, 20, 40, 200):
+        x = rows(m, k, torch.bfloat16, m)
+        out = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+        kernels.gemm_fp8(x, w, sw, out)
+        xc, sx = quantized(x)
+        want, mag = expect(xc, sx, tail, st)
+        check_product(out[:, first:first + 300], want, mag, k)
+        assert bool((out[:, :first] == 0).all()) and bool((out[:, first + 300:] == 0).all())
+    del w, out
+    x = torch.zeros(n, k, dtype=torch.bfloat16, device="cuda")
+    x[-5:] = rows(5, k, torch.bfloat16, 9)
+    codes, scales = kernels.fp8_empty(n, k, "cuda"), torch.empty(n, 64, device="cuda")
+    kernels.fp8_quantize_rows(x, codes, scales)
+    want, ws = codes_of(x[-5:])
+    assert same(codes[-5:], want) and torch.equal(scales[-5:].double(), ws) and bool((scales[:-5] == 1).all())
+    kernels.fp8_quantize_blocks(x, codes, scales := torch.empty(-(-n // 128), 64, device="cuda"))
+    want, ws = codes_of(x[n - n % 128 if n % 128 else n - 128:], 128)
+    assert same(codes[n - want.shape[0]:], want) and torch.equal(scales[-1:].double(), ws)
+
+
 def test_out_shares_no_memory_with_an_operand():
     k = 256
     w, sw = quantized(rows(256, k, torch.bfloat16, 1, wide=False), 128)

@@ -207,6 +207,26 @@ def test_numbers_that_are_none():
     agree(out, want, bound)
 
 
+def test_offsets_beyond_32_bits():
+    n_slots, v = 17_000, 128_256                       # 2.2e9 counts
+    counts = torch.zeros(n_slots, v, dtype=torch.int32, device="cuda")
+    seen = torch.zeros(n_slots, words(v), dtype=torch.int32, device="cuda")
+    slots = torch.tensor([n_slots - 1, n_slots - 2], dtype=torch.int32, device="cuda")
+    tokens = torch.tensor([5, v - 1, 5, 7], dtype=torch.int32, device="cuda")
+    kernels.history_append(counts, seen, tokens, slots, torch.tensor([0, 3, 4], dtype=torch.int32, device="cuda"))
+    assert int(counts[-1, 5]) == 2 and int(counts[-1, v - 1]) == 1 and int(counts[-2, 7]) == 1 and int(counts.sum(dtype=torch.int64)) == 4
+    m = 17_000
+    logits = torch.ones(m, v, device="cuda")
+    at = torch.full((m,), -1, dtype=torch.int32, device="cuda")
+    at[-1] = n_slots - 1
+    pen = torch.tensor([[2.0, 0.25, 0.5]], device="cuda").repeat(m, 1)
+    kernels.adjust_logits(logits, logits, at, pen, counts, seen)
+    assert logits[-1, 5].item() == 0.5 - 1.25 and logits[-1, v - 1].item() == 0.5 - 0.75
+    assert int((logits != 1).sum()) == 2
+    kernels.history_reset(counts, seen, slots)
+    assert int(counts.sum(dtype=torch.int64)) == 0 and int(seen.sum(dtype=torch.int64)) == 0
+
+
 def test_captured_with_the_history_that_moves_on():
     n, v, n_slots = 4, 5000, 6
     a = case(n, v, torch.float32, 5, biases=False, masks=False, n_slots=n_slots)
