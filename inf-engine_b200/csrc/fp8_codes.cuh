@@ -14,6 +14,17 @@ template <> struct Raw8<bf16> {
   __device__ __forceinline__ void load(const bf16* __restrict__ row, int col, int cols, bool vec) {
     if (vec && col + 8 <= cols) {
       u = *reinterpret_cast<const uint4*>(row + col);
+    } else if (col + 8 <= cols) {
+      // a row that starts anywhere: whole words, and where it starts between two, halves at both ends
+      const uint16_t* at = reinterpret_cast<const uint16_t*>(row + col);
+      if (((uintptr_t)at & 2) == 0) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(at);
+        u = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(at + 1);
+        const uint32_t first = at[0], a = w[0], b = w[1], c = w[2], last = at[7];
+        u = make_uint4(first | a << 16, __byte_perm(a, b, 0x5432), __byte_perm(b, c, 0x5432), c >> 16 | last << 16);
+      }
     } else {
       uint32_t h[8];
 #pragma unroll
