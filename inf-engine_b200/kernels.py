@@ -1881,7 +1881,7 @@ def fp8_quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
     """x (float32 or bfloat16 [n, k]) as 8-bit floating point with a scale for each row and 128 columns:
     ``codes`` (float8_e4m3fn [n, k], rows a multiple of 16 bytes apart) times ``scales`` (float32 [n, ceil(k / 128)], any strides).
     A scale is the least power of two that brings the group's largest finite number to at most 448 (1 for zeros); a code is
-    the nearest e4m3 number to x / scale, ties to even, NaN for a number that is not finite."""
+    the nearest e4m3 number to x / scale, ties to even, NaN for a number that is not finite.  The three share no memory."""
     what = "fp8_quantize_rows"
     code = _rows_in(what, "x", x)
     n, k, pitch = _codes(what, "codes", codes)
@@ -1889,12 +1889,15 @@ def fp8_quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
         _refuse(what, "codes has another shape than x")
     if scales.shape != (n, (k + 127) // 128) or scales.dtype is not _F32:
         _refuse(what, "scales is float32 [n, ceil(k / 128)]")
+    at, to, ldx = x.data_ptr(), codes.data_ptr(), x.stride(0)
+    if n and at < to + (n - 1) * pitch + k and to < at + _BYTES[code] * ((n - 1) * ldx + k) and _overlap(x, codes):
+        _refuse(what, "codes shares memory with x")
     dev = _here(x)
     if not dev == codes.get_device() == scales.get_device():
         _away(what, x, codes, scales)
     s_row, s_col = scales.stride()
-    _check(fp8_library().ie_fp8_quantize_rows(x.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), n, k, x.stride(0), pitch, s_row,
-                                              s_col, _stream_of(dev)), what)
+    _check(fp8_library().ie_fp8_quantize_rows(at, code, to, scales.data_ptr(), n, k, ldx, pitch, s_row, s_col,
+                                              _stream_of(dev)), what)
 
 
 def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
@@ -1907,11 +1910,13 @@ def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
         _refuse(what, "codes has another shape than w")
     if scales.shape != ((n + 127) // 128, (k + 127) // 128) or scales.dtype is not _F32 or not scales.is_contiguous():
         _refuse(what, "scales is a contiguous float32 [ceil(n / 128), ceil(k / 128)]")
+    at, to, ldw = w.data_ptr(), codes.data_ptr(), w.stride(0)
+    if n and at < to + (n - 1) * pitch + k and to < at + _BYTES[code] * ((n - 1) * ldw + k) and _overlap(w, codes):
+        _refuse(what, "codes shares memory with w")
     dev = _here(w)
     if not dev == codes.get_device() == scales.get_device():
         _away(what, w, codes, scales)
-    _check(fp8_library().ie_fp8_quantize_blocks(w.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), n, k, w.stride(0), pitch,
-                                                _stream_of(dev)), what)
+    _check(fp8_library().ie_fp8_quantize_blocks(at, code, to, scales.data_ptr(), n, k, ldw, pitch, _stream_of(dev)), what)
 
 
 def gemm_fp8_scratch_bytes(x: torch.Tensor) -> int:
@@ -1927,7 +1932,7 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
     float32 / bfloat16 rows, which are quantised as ``fp8_quantize_rows`` does.  Codes lie as ``fp8_empty`` lays them out.  Sums are
     float32: inside a block of 128 columns on the tensor cores, over the scaled blocks in registers.  ``out`` shares no memory with
     the operands.  ``scratch`` (uint8, at least ``gemm_fp8_scratch_bytes(x)``) takes the codes of rows that are quantised here;
-    without it they go into memory of this call's own."""
+    without it they go into memory of this call's own.  It lies apart from the operands and ``out``."""
     what = "gemm_fp8"
     n, k, w_pitch = _codes(what, "w", w)
     code, to = _OPERANDS.get(x.dtype), _CODES.get(out.dtype)
@@ -1978,6 +1983,11 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
         if scratch.dtype is not torch.uint8 or not scratch.is_contiguous() or scratch.data_ptr() % 16 or scratch.get_device() != dev:
             _refuse(what, "scratch is contiguous bytes that start on 16, beside the operands")
         room = scratch.data_ptr()
+        # kernels that quantise the rows ahead read x and write scratch, and the product reads scratch and writes out
+        ends = room + size
+        if ((room < end and y < ends) or (room < at + _BYTES[code] * ((m - 1) * ldx + k) and at < ends)
+                or (room < of + (n - 1) * w_pitch + k and of < ends)):
+            _refuse(what, "scratch shares memory with the operands or out")
     elif code != IE_E4M3 and (m > 8 or code == IE_F32):                # few bfloat16 rows may need none: the call says so
         own = x.new_empty(gemm_fp8_scratch_bytes(x), dtype=torch.uint8)
         room, size = own.data_ptr(), own.numel()

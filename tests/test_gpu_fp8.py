@@ -251,6 +251,21 @@ def test_out_shares_no_memory_with_an_operand():
         kernels.gemm_fp8(x, w, sw, torch.empty(20, 256, device="cuda"), scratch=small)
 
 
+def test_scratch_lies_apart():
+    k = 256
+    w, sw = quantized(rows(256, k, torch.bfloat16, 1, wide=False), 128)
+    out = torch.empty(20, 256, device="cuda")
+    buf = torch.empty(64 << 10, dtype=torch.uint8, device="cuda")
+    x = buf[:20 * k * 2].view(torch.bfloat16).view(20, k)
+    x.copy_(rows(20, k, torch.bfloat16, 2))
+    bytes_ = kernels.gemm_fp8_scratch_bytes(x)
+    for scratch in (buf[:bytes_], buf[20 * k * 2 - 16:], out.view(torch.uint8).view(-1), w.view(torch.uint8).view(-1)):
+        with pytest.raises(kernels.KernelError, match="scratch shares memory"):
+            kernels.gemm_fp8(x, w, sw, out, scratch=scratch)
+    kernels.gemm_fp8(x, w, sw, out, scratch=buf[20 * k * 2:20 * k * 2 + bytes_])
+    check_product(out, *expect(*quantized(x), w, sw), k)
+
+
 FIRST = """
 import torch
 from inf_engine_b200 import kernels

@@ -106,3 +106,20 @@ def test_adjust():
     refused("current device", f, x, out, **p, **b, **m)
     # side by side in one buffer is no overlap: the refusal is the device's
     refused("current device", f, torch.as_strided(buf, (3, 100), (250, 1)), torch.as_strided(buf, (3, 100), (250, 1), 120))
+
+
+@pytest.mark.parametrize("name,high", [("fp8_quantize_rows", 1), ("fp8_quantize_blocks", 128)])
+def test_codes_lie_apart_from_what_they_come_from(name, high):
+    f = getattr(kernels, name)
+    buf = torch.zeros(4 * 1024, dtype=torch.uint8)
+    scales = torch.zeros(-(-4 // high), 2)
+    x = buf.view(torch.bfloat16)[:4 * 200].view(4, 200)
+    codes = buf.view(kernels.FP8)
+    refused("shares memory", f, x, torch.as_strided(codes, (4, 200), (208, 1)), scales)
+    refused("shares memory", f, x, torch.as_strided(codes, (4, 200), (208, 1), 16 * 99), scales)     # x ends behind 1,600 bytes
+    refused("current device", f, x, torch.as_strided(codes, (4, 200), (208, 1), 1600), scales)
+    refused("current device", f, buf.view(torch.float32)[:800].view(4, 200)[:0], torch.as_strided(codes, (4, 200), (208, 1))[:0], scales[:0])
+    # side by side in rows of 1,024 bytes
+    rows = torch.as_strided(buf.view(torch.bfloat16), (4, 200), (512, 1))
+    refused("current device", f, rows, torch.as_strided(codes, (4, 200), (1024, 1), 512), scales)
+    refused("shares memory", f, rows, torch.as_strided(codes, (4, 200), (1024, 1), 384), scales)
