@@ -48,6 +48,11 @@ template <> struct Raw8<float> {
     if (vec && col + 8 <= cols) {
       a = *reinterpret_cast<const float4*>(row + col);
       b = *reinterpret_cast<const float4*>(row + col + 4);
+    } else if (col + 8 <= cols && ((uintptr_t)(row + col) & 7) == 0) {
+      const float2* at = reinterpret_cast<const float2*>(row + col);
+      const float2 c = at[0], d = at[1], e = at[2], f = at[3];
+      a = make_float4(c.x, c.y, d.x, d.y);
+      b = make_float4(e.x, e.y, f.x, f.y);
     } else {
       float v[8];
 #pragma unroll

@@ -12,8 +12,9 @@
 // Both read every number once and write a byte for it; the HBM rate is the bound: 4,096 rows of 8,192 in bfloat16 take 18.4 us (5.5
 // TB/s), in float32 25.7 (6.5), a weight of 16,384 x 2,048 in bfloat16 19.1 us (5.3).  With a look at every number for infinities
 // (now only where a group's largest is one) and 8 numbers a lane the bfloat16 rows took 28 us: instructions.
-// Rows that do not start on 16 bytes are read by words: 4,096 x 8,190 in bfloat16 takes 28.7 us, 8,191 (every other row starts
-// between two words) 32.8; number by number both took 39.
+// Rows that do not start on 16 bytes, caches flushed (24.5 and 32.8 us where they do): 4,096 x 8,190 in bfloat16, by words, takes 28.7 us,
+// 8,191 (every other row starts between two words) 32.8; in float32, by pairs where a row starts on one, 36.9 and 43.0; number by
+// number 38.9 in bfloat16, 49.2 in float32.
 #include "fp8_codes.cuh"
 
 namespace {
