@@ -121,8 +121,8 @@ inline int reads_vectors(const void* x, long long ld, int dtype) {
 
 // x [rows, cols] (dtype: IE_F32 or IE_BF16, row pitch ldx elements) -> codes [rows, cols] (row pitch ldc bytes, a multiple of 16) and
 // scales[row * s_row + group * s_col].  Bytes between the rows of codes are left as they are.
-extern "C" int ie_fp8_quantize_rows(const void* x, int dtype, void* codes, float* scales, int rows, int cols, long long ldx,
-                                    long long ldc, long long s_row, long long s_col, cudaStream_t stream) {
+int fp8_quantize_rows(const void* x, int dtype, void* codes, float* scales, int rows, int cols, long long ldx, long long ldc,
+                      long long s_row, long long s_col, cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return IE_OK;
   if (dtype != IE_F32 && dtype != IE_BF16) return IE_BAD_DTYPE;
   if (((uintptr_t)codes & 15) || ldc % 16) return IE_BAD_ALIGN;
@@ -141,8 +141,8 @@ extern "C" int ie_fp8_quantize_rows(const void* x, int dtype, void* codes, float
 }
 
 // w [rows, cols] -> codes and scales [ceil(rows / 128), ceil(cols / 128)], contiguous
-extern "C" int ie_fp8_quantize_blocks(const void* w, int dtype, void* codes, float* scales, int rows, int cols, long long ldw,
-                                      long long ldc, cudaStream_t stream) {
+static int fp8_quantize_blocks(const void* w, int dtype, void* codes, float* scales, int rows, int cols, long long ldw, long long ldc,
+                               cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return IE_OK;
   if (dtype != IE_F32 && dtype != IE_BF16) return IE_BAD_DTYPE;
   if (((uintptr_t)codes & 15) || ldc % 16) return IE_BAD_ALIGN;
@@ -152,4 +152,14 @@ extern "C" int ie_fp8_quantize_blocks(const void* w, int dtype, void* codes, flo
   if (dtype == IE_F32)
     return launch_k(quantize_blocks_kernel<float>, grid, BT, 0, stream, (const float*)w, (uint8_t*)codes, scales, rows, cols, ldw, ldc, vec);
   return launch_k(quantize_blocks_kernel<bf16>, grid, BT, 0, stream, (const bf16*)w, (uint8_t*)codes, scales, rows, cols, ldw, ldc, vec);
+}
+
+// the entries: arguments as 64-bit words in the order above, which a caller converts in one go; sizes of 2^31 and more are refused
+extern "C" int ie_fp8_quantize_rows(const long long* a) {
+  if ((a[4] | a[5]) >> 31) return IE_BAD_SIZE;
+  return fp8_quantize_rows((const void*)a[0], (int)a[1], (void*)a[2], (float*)a[3], (int)a[4], (int)a[5], a[6], a[7], a[8], a[9], (cudaStream_t)a[10]);
+}
+extern "C" int ie_fp8_quantize_blocks(const long long* a) {
+  if ((a[4] | a[5]) >> 31) return IE_BAD_SIZE;
+  return fp8_quantize_blocks((const void*)a[0], (int)a[1], (void*)a[2], (float*)a[3], (int)a[4], (int)a[5], a[6], a[7], (cudaStream_t)a[8]);
 }

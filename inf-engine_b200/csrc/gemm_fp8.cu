@@ -5,7 +5,7 @@
 //
 // inner and outer sums in float32, one rounding to the output's type.
 //
-// Four kernels, by the rows of x and the length of the weight (ie_gemm_fp8 holds the rules, with both sides measured):
+// Four kernels, by the rows of x and the length of the weight (gemm_fp8 at the end holds the rules, with both sides measured):
 //   few rows          registers and the matrix instructions for halves; bfloat16 rows may be quantised inside
 //   a long weight     under up to 32 rows: the tensor cores, w as the larger operand, bound by the weight's bytes (5.6 TB/s)
 //   tiles             128 x 128, K dealt out over a cluster where tiles are few
@@ -1068,8 +1068,8 @@ int launch_few(const Fp8Params& p, int sms, cudaStream_t stream) {
 }  // namespace
 
 // fp8_quantize.cu
-extern "C" int ie_fp8_quantize_rows(const void* x, int dtype, void* codes, float* scales, int rows, int cols, long long ldx,
-                                    long long ldc, long long s_row, long long s_col, cudaStream_t stream);
+int fp8_quantize_rows(const void* x, int dtype, void* codes, float* scales, int rows, int cols, long long ldx, long long ldc,
+                      long long s_row, long long s_col, cudaStream_t stream);
 
 // bytes of scratch that the product of unquantised rows takes, unless it quantises them itself: their codes, then their scales [K / 128][M]
 static long long scratch_of(int M, int K) {
@@ -1078,9 +1078,9 @@ static long long scratch_of(int M, int K) {
 }
 
 // x: codes (x_dtype IE_E4M3, with sx) or float32 / bfloat16 rows, which are quantised into scratch first
-extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const void* w, const float* sw, void* y, int y_dtype, int M,
-                           int N, int K, long long ldx, long long sx_row, long long sx_col, long long ldw, long long ldy,
-                           void* scratch, long long scratch_bytes, cudaStream_t stream) {
+static int gemm_fp8(const void* x, int x_dtype, const float* sx, const void* w, const float* sw, void* y, int y_dtype, int M, int N, int K,
+                    long long ldx, long long sx_row, long long sx_col, long long ldw, long long ldy, void* scratch,
+                    long long scratch_bytes, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return IE_OK;
   if (K <= 0) return IE_BAD_SIZE;
   if (y_dtype != IE_F32 && y_dtype != IE_BF16) return IE_BAD_DTYPE;
@@ -1106,7 +1106,7 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
     if ((uintptr_t)scratch & 15) return IE_BAD_ALIGN;
     const long long pitch = (K + 15) / 16 * 16;
     float* scales = reinterpret_cast<float*>((char*)scratch + M * pitch);
-    const int rc = ie_fp8_quantize_rows(x, x_dtype, scratch, scales, M, K, ldx, pitch, 1, M, stream);
+    const int rc = fp8_quantize_rows(x, x_dtype, scratch, scales, M, K, ldx, pitch, 1, M, stream);
     if (rc) return rc;
     x = scratch; ldx = pitch; sx = scales; sx_row = 1; sx_col = M;
     p.early = 1;
@@ -1126,6 +1126,13 @@ extern "C" int ie_gemm_fp8(const void* x, int x_dtype, const float* sx, const vo
   static FitTable fits;
   p.split = blocks_a_tile(gemm_fp8_tile_kernel<false, true>, TILE_THREADS, (int)TILE_SMEM, tiles, (K + GROUP - 1) / GROUP, 4, fits);
   return p.split > 1 ? launch_tiles<false, true>(p, sms, stream) : launch_tiles<false, false>(p, sms, stream);
+}
+
+// the entry: arguments as 64-bit words in the order above, which a caller converts in one go; sizes of 2^31 and more are refused
+extern "C" int ie_gemm_fp8(const long long* a) {
+  if ((a[7] | a[8] | a[9]) >> 31) return IE_BAD_SIZE;
+  return gemm_fp8((const void*)a[0], (int)a[1], (const float*)a[2], (const void*)a[3], (const float*)a[4], (void*)a[5], (int)a[6], (int)a[7],
+                  (int)a[8], (int)a[9], a[10], a[11], a[12], a[13], a[14], (void*)a[15], a[16], (cudaStream_t)a[17]);
 }
 
 // reads and clears the word that a wait which ran out leaves (0: none)

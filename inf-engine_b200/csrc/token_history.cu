@@ -218,25 +218,25 @@ __global__ void __launch_bounds__(HT, 8) adjust_logits_kernel(AdjustParams p) {
 
 }  // namespace
 
-extern "C" int ie_history_reset(int* counts, int* seen, const int* slots, int n, int n_slots, int vocab, cudaStream_t stream) {
+static int history_reset(int* counts, int* seen, const int* slots, int n, int n_slots, int vocab, cudaStream_t stream) {
   if (n <= 0 || vocab <= 0 || n_slots <= 0) return IE_OK;
   if (n > 65535) return IE_BAD_SIZE;
   const int blocks = (vocab + 32 * HT - 1) / (32 * HT);       // eight stores of 16 bytes a thread
   return launch_k(history_reset_kernel, dim3(blocks, n), HT, 0, stream, counts, seen, slots, n_slots, vocab, (vocab + 31) / 32);
 }
 
-extern "C" int ie_history_append(int* counts, int* seen, const int* tokens, const int* slots, const int* starts, const int* n_prompt,
-                                 int n_tokens, int n_requests, int n_slots, int vocab, cudaStream_t stream) {
+static int history_append(int* counts, int* seen, const int* tokens, const int* slots, const int* starts, const int* n_prompt,
+                          int n_tokens, int n_requests, int n_slots, int vocab, cudaStream_t stream) {
   if (n_tokens <= 0 || n_requests <= 0 || vocab <= 0 || n_slots <= 0) return IE_OK;
   if (starts == nullptr && n_tokens != n_requests) return IE_BAD_SIZE;
   return launch_k(history_append_kernel, (n_tokens + HT - 1) / HT, HT, 0, stream, counts, seen, tokens, slots, starts, n_prompt,
                   n_tokens, n_requests, n_slots, vocab, (vocab + 31) / 32);
 }
 
-extern "C" int ie_adjust_logits(const void* logits, int dtype, float* out, const int* slots, const float* penalties, const int* counts,
-                                const int* seen, const int* bias_start, const int* bias_ids, const float* bias_values,
-                                const int* mask_rows, const int* masks, int n_rows, int vocab, long long ld_in, long long ld_out,
-                                int n_slots, int n_bias, int n_masks, int in_place, cudaStream_t stream) {
+static int adjust_logits(const void* logits, int dtype, float* out, const int* slots, const float* penalties, const int* counts,
+                         const int* seen, const int* bias_start, const int* bias_ids, const float* bias_values,
+                         const int* mask_rows, const int* masks, int n_rows, int vocab, long long ld_in, long long ld_out,
+                         int n_slots, int n_bias, int n_masks, int in_place, cudaStream_t stream) {
   if (n_rows <= 0 || vocab <= 0) return IE_OK;
   if (n_rows > 65535) return IE_BAD_SIZE;
   if (dtype != IE_F32 && dtype != IE_BF16) return IE_BAD_DTYPE;
@@ -257,4 +257,21 @@ extern "C" int ie_adjust_logits(const void* logits, int dtype, float* out, const
   if (dtype == IE_F32)
     return vec ? launch_k(adjust_logits_kernel<float, 4>, grid, HT, 0, stream, p) : launch_k(adjust_logits_kernel<float, 1>, grid, HT, 0, stream, p);
   return vec ? launch_k(adjust_logits_kernel<bf16, 4>, grid, HT, 0, stream, p) : launch_k(adjust_logits_kernel<bf16, 1>, grid, HT, 0, stream, p);
+}
+
+// the entries: arguments as 64-bit words in the order above, which a caller converts in one go; sizes of 2^31 and more are refused
+extern "C" int ie_history_reset(const long long* a) {
+  if ((a[3] | a[4] | a[5]) >> 31) return IE_BAD_SIZE;
+  return history_reset((int*)a[0], (int*)a[1], (const int*)a[2], (int)a[3], (int)a[4], (int)a[5], (cudaStream_t)a[6]);
+}
+extern "C" int ie_history_append(const long long* a) {
+  if ((a[6] | a[7] | a[8] | a[9]) >> 31) return IE_BAD_SIZE;
+  return history_append((int*)a[0], (int*)a[1], (const int*)a[2], (const int*)a[3], (const int*)a[4], (const int*)a[5], (int)a[6],
+                        (int)a[7], (int)a[8], (int)a[9], (cudaStream_t)a[10]);
+}
+extern "C" int ie_adjust_logits(const long long* a) {
+  if ((a[12] | a[13] | a[16] | a[17] | a[18]) >> 31) return IE_BAD_SIZE;
+  return adjust_logits((const void*)a[0], (int)a[1], (float*)a[2], (const int*)a[3], (const float*)a[4], (const int*)a[5],
+                       (const int*)a[6], (const int*)a[7], (const int*)a[8], (const float*)a[9], (const int*)a[10], (const int*)a[11],
+                       (int)a[12], (int)a[13], a[14], a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19], (cudaStream_t)a[20]);
 }
