@@ -123,3 +123,21 @@ def test_codes_lie_apart_from_what_they_come_from(name, high):
     rows = torch.as_strided(buf.view(torch.bfloat16), (4, 200), (512, 1))
     refused("current device", f, rows, torch.as_strided(codes, (4, 200), (1024, 1), 512), scales)
     refused("shares memory", f, rows, torch.as_strided(codes, (4, 200), (1024, 1), 384), scales)
+
+
+def test_launchers_refuse_sizes_that_pass_32_bits():
+    """Before anything is launched, so this runs without a GPU."""
+    big, bad_size = 1 << 31, -2
+    fp8, core = kernels.fp8_library(), kernels.core()
+    for at in (4, 5):
+        size = [big if i == at else 1 for i in range(11)]
+        assert fp8.ie_fp8_quantize_rows(kernels._11_words(*size)) == bad_size
+        assert fp8.ie_fp8_quantize_blocks(kernels._9_words(*size[:9])) == bad_size
+    for at in (7, 8, 9):
+        assert fp8.ie_gemm_fp8(kernels._18_words(*[big if i == at else 1 for i in range(18)])) == bad_size
+    for at in (3, 4, 5):
+        assert core.ie_history_reset(kernels._7_words(*[big if i == at else 1 for i in range(7)])) == bad_size
+    for at in (6, 7, 8, 9):
+        assert core.ie_history_append(kernels._11_words(*[big if i == at else 1 for i in range(11)])) == bad_size
+    for at in (12, 13, 16, 17, 18):
+        assert core.ie_adjust_logits(kernels._21_words(*[big if i == at else 1 for i in range(21)])) == bad_size
