@@ -1,5 +1,9 @@
 """What the 8-bit products, request histories and adjusted logits refuse, before anything reaches a GPU."""
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -125,19 +129,28 @@ def test_codes_lie_apart_from_what_they_come_from(name, high):
     refused("shares memory", f, rows, torch.as_strided(codes, (4, 200), (1024, 1), 384), scales)
 
 
+SIZES = """
+from inf_engine_b200 import kernels
+big, bad_size = 1 << 31, -2
+def words(pack, n, at):
+    return pack(*[big if i == at else 1 for i in range(n)])
+fp8, core = kernels.fp8_library(), kernels.core()
+for at in (4, 5):
+    assert fp8.ie_fp8_quantize_rows(words(kernels._11_words, 11, at)) == bad_size
+    assert fp8.ie_fp8_quantize_blocks(words(kernels._9_words, 9, at)) == bad_size
+for at in (7, 8, 9):
+    assert fp8.ie_gemm_fp8(words(kernels._18_words, 18, at)) == bad_size
+for at in (3, 4, 5):
+    assert core.ie_history_reset(words(kernels._7_words, 7, at)) == bad_size
+for at in (6, 7, 8, 9):
+    assert core.ie_history_append(words(kernels._11_words, 11, at)) == bad_size
+for at in (12, 13, 16, 17, 18):
+    assert core.ie_adjust_logits(words(kernels._21_words, 21, at)) == bad_size
+"""
+
+
 def test_launchers_refuse_sizes_that_pass_32_bits():
-    """Before anything is launched, so this runs without a GPU."""
-    big, bad_size = 1 << 31, -2
-    fp8, core = kernels.fp8_library(), kernels.core()
-    for at in (4, 5):
-        size = [big if i == at else 1 for i in range(11)]
-        assert fp8.ie_fp8_quantize_rows(kernels._11_words(*size)) == bad_size
-        assert fp8.ie_fp8_quantize_blocks(kernels._9_words(*size[:9])) == bad_size
-    for at in (7, 8, 9):
-        assert fp8.ie_gemm_fp8(kernels._18_words(*[big if i == at else 1 for i in range(18)])) == bad_size
-    for at in (3, 4, 5):
-        assert core.ie_history_reset(kernels._7_words(*[big if i == at else 1 for i in range(7)])) == bad_size
-    for at in (6, 7, 8, 9):
-        assert core.ie_history_append(kernels._11_words(*[big if i == at else 1 for i in range(11)])) == bad_size
-    for at in (12, 13, 16, 17, 18):
-        assert core.ie_adjust_logits(kernels._21_words(*[big if i == at else 1 for i in range(21)])) == bad_size
+    """Before anything is launched, so this runs without a GPU; in a process of its own, which loads the libraries."""
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", SIZES], cwd=root, capture_output=True, text=True, timeout=900)
+    assert r.returncode == 0, r.stderr[-2000:]
