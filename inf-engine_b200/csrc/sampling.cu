@@ -14,6 +14,11 @@
 //           the inverse CDF in vocabulary order at a uniform number that is a
 //           hash of (seed, key): it depends on the request and its position
 //           only, not on what else is in the batch.
+//
+// A token is answered only if it has a share of the draw: -inf (a masked token), NaN, and a number so far below the
+// largest that exp gives 0 have none, also where the walk ends by rounding (it then answers the last token that has
+// one).  NaN counts as -inf everywhere.  A row whose largest logit is +inf, or becomes infinite when it is divided by the
+// temperature, answers the largest as a greedy row does, and a row with nothing above -inf answers token 0.
 #include "common.cuh"
 
 #define SM_THREADS 1024
@@ -25,10 +30,16 @@ struct SampleRow {
   unsigned int seed_lo, seed_hi, key_lo, key_hi;
 };
 
+// larger float <=> larger key.  Whole words throughout: a sign set by negating a float moves a NaN to -0's key
 __device__ __forceinline__ unsigned int order_key(float x) {
-  unsigned int u = __float_as_uint(x);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);   // larger float <=> larger key
+  const int u = __float_as_int(x);
+  return (unsigned int)((u >> 31 | (int)0x80000000) ^ u);
 }
+// keys of the least finite float and of +inf: -inf lies below them, NaN below or above
+#define KEY_LEAST 0x00800000u
+#define KEY_MOST 0xff800000u
+// whether a key is above `below` and no NaN's, below <= KEY_MOST: one comparison, as the loops over a vocabulary pay for each
+__device__ __forceinline__ bool key_above(unsigned int key, unsigned int below) { return key - below - 1u < KEY_MOST - below; }
 
 __device__ __forceinline__ unsigned long long splitmix64(unsigned long long x) {
   x += 0x9E3779B97F4A7C15ull;
@@ -67,7 +78,7 @@ __global__ void __launch_bounds__(SM_THREADS) argmax_kernel(const float* __restr
   int best_i = 0x7fffffff;
   for (int i = threadIdx.x; i < vocab; i += blockDim.x) {
     const float v = x[i];
-    if (v > best || (v == best && i < best_i) || best_i == 0x7fffffff) { best = v; best_i = i; }
+    if (v > best) { best = v; best_i = i; }            // -inf and NaN never: a thread that sees nothing else has no index
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -143,9 +154,12 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ x, const Sa
   float best = -INFINITY;
   for (int i = tid; i < vocab; i += SM_THREADS) best = fmaxf(best, x[i]);
   best = block_max(best, red);
-  if (r.temperature <= 0.f) {
+  const float temperature = fminf(r.temperature, 3.402823466e38f);      // -inf divided by it stays -inf
+  float m = INFINITY;
+  if (temperature > 0.f) m = best / temperature;
+  if (!(m > -INFINITY && m < INFINITY)) {
     int first = 0x7fffffff;
-    for (int i = tid; i < vocab; i += SM_THREADS)
+    for (int i = best > -INFINITY ? tid : vocab; i < vocab; i += SM_THREADS)
       if (x[i] == best) { first = i; break; }
     // minimum over the block
 #pragma unroll
@@ -161,20 +175,22 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ x, const Sa
     }
     return;
   }
-  const float m = best / r.temperature;
 
-  // top-k: the key of the k-th largest scaled logit, bit by bit from the top
-  unsigned int key_floor = 0u;   // keep keys >= key_floor
+  // top-k: the key of the k-th largest scaled logit, bit by bit from the top; NaN, whose key lies above, comes on top of k
+  unsigned int below = KEY_LEAST - 1u;   // keep keys above it
   if (r.top_k > 0 && r.top_k < vocab) {
+    int nans = 0;
+    for (int i = tid; i < vocab; i += SM_THREADS) nans += x[i] != x[i];
+    const int k = r.top_k + block_sum_int(nans, redi);
     unsigned int prefix = 0u;
     for (int bit = 31; bit >= 0; --bit) {
       const unsigned int cand = prefix | (1u << bit);
       int cnt = 0;
-      for (int i = tid; i < vocab; i += SM_THREADS) cnt += order_key(x[i] / r.temperature) >= cand;
+      for (int i = tid; i < vocab; i += SM_THREADS) cnt += order_key(x[i] / temperature) >= cand;
       cnt = block_sum_int(cnt, redi);
-      if (cnt >= r.top_k) prefix = cand;   // at least k keys are >= cand: the k-th largest is too
+      if (cnt >= k) prefix = cand;   // at least k keys are >= cand: the k-th largest is too
     }
-    key_floor = prefix;
+    below = max(below, max(prefix, 1u) - 1u);
   }
 
   // top-p over what top-k left: the largest key K with mass(keys > K) < p keeps
@@ -182,8 +198,8 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ x, const Sa
   if (r.top_p < 1.0f) {
     float z = 0.f;
     for (int i = tid; i < vocab; i += SM_THREADS) {
-      const float s = x[i] / r.temperature;
-      if (order_key(s) >= key_floor) z += expf(s - m);
+      const float s = x[i] / temperature;
+      if (key_above(order_key(s), below)) z += expf(s - m);
     }
     z = block_sum(z, red);
     const float budget = r.top_p * z;
@@ -191,17 +207,16 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ x, const Sa
     // K has a bit cleared when clearing it still leaves mass(keys > K) < budget
     unsigned int K = 0xffffffffu;
     for (int bit = 31; bit >= 0; --bit) {
-      const unsigned int cand = K & ~(1u << bit);
+      const unsigned int cand = K & ~(1u << bit), over = min(max(cand, below), KEY_MOST);
       float above = 0.f;
       for (int i = tid; i < vocab; i += SM_THREADS) {
-        const float s = x[i] / r.temperature;
-        const unsigned int k = order_key(s);
-        if (k > cand && k >= key_floor) above += expf(s - m);
+        const float s = x[i] / temperature;
+        if (key_above(order_key(s), over)) above += expf(s - m);
       }
       above = block_sum(above, red);
       if (above < budget) K = cand;
     }
-    key_floor = max(key_floor, K);
+    below = max(below, max(K, 1u) - 1u);      // the largest number is above it: the budget is more than nothing
   }
 
   // inverse CDF in vocabulary order over the kept tokens
@@ -209,8 +224,8 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ x, const Sa
   const int lo = tid * per, hi = min(vocab, lo + per);
   float mine = 0.f;
   for (int i = lo; i < hi; ++i) {
-    const float s = x[i] / r.temperature;
-    if (order_key(s) >= key_floor) mine += expf(s - m);
+    const float s = x[i] / temperature;
+    if (key_above(order_key(s), below)) mine += expf(s - m);
   }
   chunk_sum[tid] = mine;
   __syncthreads();
@@ -228,22 +243,25 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ x, const Sa
       if (run + chunk_sum[t] > target) break;
       run += chunk_sum[t];
     }
-    // walk the chunk; the last kept token catches rounding at the very end
+    // walk the chunk; the last token with a share catches rounding at the very end
     int pick = -1, last_kept = -1;
     for (int tt = t; tt < SM_THREADS && pick < 0; ++tt) {
       const int l2 = tt * per, h2 = min(vocab, l2 + per);
       for (int i = l2; i < h2; ++i) {
-        const float s = x[i] / r.temperature;
-        if (order_key(s) < key_floor) continue;
-        last_kept = i;
-        run += expf(s - m);
+        const float s = x[i] / temperature;
+        if (!key_above(order_key(s), below)) continue;
+        const float w = expf(s - m);
+        if (w > 0.f) last_kept = i;
+        run += w;
         if (run > target) { pick = i; break; }
       }
     }
     if (pick < 0) {
       if (last_kept < 0)
-        for (int i = vocab - 1; i >= 0; --i)
-          if (order_key(x[i] / r.temperature) >= key_floor) { last_kept = i; break; }
+        for (int i = vocab - 1; i >= 0; --i) {
+          const float s = x[i] / temperature;
+          if (key_above(order_key(s), below) && expf(s - m) > 0.f) { last_kept = i; break; }
+        }
       pick = last_kept < 0 ? 0 : last_kept;
     }
     *out = pick;
@@ -304,13 +322,13 @@ __global__ void __launch_bounds__(SM_THREADS) greedy_split_kernel(const float* _
     for (int k = 0; k < 4; ++k) v[k] = (i0 + k * SM_THREADS < hi) ? x[i0 + k * SM_THREADS] : -INFINITY;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (i0 + k * SM_THREADS < hi && (v[k] > cb[k] || ci[k] == 0x7fffffff)) { cb[k] = v[k]; ci[k] = i0 + k * SM_THREADS; }
+      if (v[k] > cb[k]) { cb[k] = v[k]; ci[k] = i0 + k * SM_THREADS; }      // -inf and NaN never
   }
   float best = cb[0];
   int best_i = ci[0];
 #pragma unroll
   for (int k = 1; k < 4; ++k)
-    if (ci[k] != 0x7fffffff && (best_i == 0x7fffffff || cb[k] > best || (cb[k] == best && ci[k] < best_i))) { best = cb[k]; best_i = ci[k]; }
+    if (cb[k] > best || (cb[k] == best && ci[k] < best_i)) { best = cb[k]; best_i = ci[k]; }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float ov = __shfl_xor_sync(0xffffffffu, best, o);
@@ -334,7 +352,7 @@ __global__ void __launch_bounds__(SM_THREADS) greedy_split_kernel(const float* _
       for (int c = 0; c < n_chunks; ++c) {
         const float v = __ldcg(&g_sg_val[row * SG_CHUNKS + c]);
         const int i = __ldcg(&g_sg_idx[row * SG_CHUNKS + c]);
-        if (i != 0x7fffffff && (v > b || bi == 0x7fffffff || (v == b && i < bi))) { b = v; bi = i; }
+        if (v > b || (v == b && i < bi)) { b = v; bi = i; }
       }
       out[row] = bi == 0x7fffffff ? 0 : bi;
       g_sg_ticket[row] = 0;
