@@ -34,6 +34,8 @@ class Engine:
                  nvtx: bool = False):
         self.runner = runner
         self.cfg = sampling or SamplingConfig()
+        if why := self._unusable(self.cfg):
+            raise ValueError(why)
         if eos_token is None:
             eos_token = getattr(runner.config, "eos_token_id", None)
         self.eos = eos_token
@@ -90,16 +92,20 @@ class Engine:
             return cls.from_dir(tmp, dtype=dtype, **kw)
 
     # ------------------------------------------------------------------ queue
+    def _unusable(self, c: SamplingConfig) -> str | None:
+        """Why these options cannot be used; None if they can.  What is refused here would end the step of every request."""
+        try:
+            c.validate()
+        except ValueError as e:
+            return str(e)
+        if any(t >= self.runner.spec.vocab_size for t in c.logit_bias or ()):
+            return f"logit_bias names a token outside the vocabulary of {self.runner.spec.vocab_size}"
+        return None
+
     def submit(self, req: Request) -> bool:
-        if req.sampling is not None and req.sampling.adjusts:
-            try:
-                req.sampling.validate()
-            except ValueError as e:
-                req.error = str(e)
-                return False
-            if any(t >= self.runner.spec.vocab_size for t in req.sampling.logit_bias or ()):
-                req.error = f"logit_bias names a token outside the vocabulary of {self.runner.spec.vocab_size}"
-                return False
+        if req.sampling is not None and (why := self._unusable(req.sampling)):
+            req.error = why
+            return False
         if not req.arrival_time:
             req.arrival_time = time.perf_counter()      # the clock that run_offline and generate step with
         return self.scheduler.submit(req)
@@ -261,7 +267,10 @@ class Engine:
                 ids = self.sampler.sample(logits, configs, keys, contexts, self.adjuster if adjust else None, adjust)
         if wanted:
             ids = ids.tolist()                                   # the step's one device-to-host read
-            sampled = {e.request.req_id: None if e.request.req_id in stuck else t for e, t in zip(wanted, ids)}
+            for e, t, words in zip(wanted, ids, allowed):
+                if words is not None and not int(words[t >> 5]) >> (t & 31) & 1:      # what the mask lets through is -inf or NaN
+                    stuck[e.request.req_id] = "no allowed token has a logit above -inf"
+            sampled = {e.request.req_id: stuck.get(e.request.req_id, t) for e, t in zip(wanted, ids)}
         for e in plan.entries:
             self.stats["decode_tokens" if len(e.tokens) == 1 and e.request.generated else "prefill_tokens"] += len(e.tokens)
         self.stats["steps"] += 1
@@ -269,15 +278,19 @@ class Engine:
         return self.scheduler.commit(plan, sampled, now)
 
     def _allowed(self, wanted):
-        """Masks of the rows whose requests hold the next token to a set, and the ids of requests that no token may continue."""
-        allowed, stuck = [], set()
+        """Masks of the rows whose requests hold the next token to a set, and why requests cannot go on, by id: no token may continue
+        one, or its function raised or returned what is no set of tokens."""
+        allowed, stuck = [], {}
         for e in wanted:
             r, words = e.request, None
-            if r.allowed_tokens is not None and (may := r.allowed_tokens(r.generated)) is not None:
-                words = allowed_words(may, self.runner.spec.vocab_size)
-                if not words.any():
-                    stuck.add(r.req_id)
-                    words = None
+            if r.allowed_tokens is not None:
+                try:
+                    may = r.allowed_tokens(r.generated)
+                    words = None if may is None else allowed_words(may, self.runner.spec.vocab_size)
+                except Exception as ex:                          # the user's function: its request ends, the others go on
+                    stuck[r.req_id] = f"allowed_tokens: {type(ex).__name__}: {ex}"
+                if words is not None and not words.any():
+                    stuck[r.req_id], words = "no token is allowed", None
             allowed.append(words)
         return allowed, stuck
 

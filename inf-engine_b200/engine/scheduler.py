@@ -48,7 +48,8 @@ class Request:
     stop_check: Callable[[list[int]], bool] | None = field(default=None, repr=False)
     sampling: SamplingConfig | None = None
     # called with the tokens generated so far before each token is chosen: the ids that may come next (or one truth value for each
-    # token of the vocabulary), None where every token may; a request that no token may continue ends with ``error`` set
+    # token of the vocabulary), None where every token may; a request that no token may continue, or whose function raises, ends with
+    # ``error`` set
     allowed_tokens: Callable[[list[int]], object] | None = field(default=None, repr=False)
     error: str | None = None
     preemptions: int = 0
@@ -243,8 +244,8 @@ class Scheduler:
     # --------------------------------------------------------------- after a step
     def commit(self, plan: StepPlan, sampled: dict, now: float = 0.0) -> list[Request]:
         """Record the step's sampled tokens (``{req_id: token}`` for the entries that
-        wanted logits; None for one that no token may continue: it ends there); finish and free what is done.  Returns the
-        requests finished."""
+        wanted logits; for one that cannot go on, None (no token is allowed) or the reason as text: it ends there); finish and free
+        what is done.  Returns the requests finished."""
         finished = []
         for e in plan.entries:
             req = e.request
@@ -253,8 +254,8 @@ class Scheduler:
             tok = sampled[req.req_id]
             if not req.generated or req.start_time == 0.0:
                 req.start_time = req.start_time or now
-            if tok is None:
-                req.error = "no token is allowed"
+            if tok is None or isinstance(tok, str):
+                req.error = tok or "no token is allowed"
                 req.finish_time = now
                 self.cache.close(req.req_id)
                 self.running.remove(req)

@@ -13,6 +13,8 @@ Differences that are on purpose:
 from __future__ import annotations
 
 import math
+import operator
+from collections.abc import Mapping
 from dataclasses import dataclass
 from enum import Enum
 
@@ -71,18 +73,37 @@ class SamplingConfig:
         return self.keeps_history or bool(self.logit_bias)
 
     def validate(self) -> None:
-        if self.mode is not SamplingMode.GREEDY and self.temperature <= 0.0:
+        """ValueError unless every option that the mode uses can be used, whatever its type."""
+        try:
+            self._validate()
+        except (TypeError, OverflowError) as e:
+            raise ValueError(f"a sampling option is not a number as it should be: {e}") from e
+
+    def _validate(self) -> None:
+        if self.mode is not SamplingMode.GREEDY and not self.temperature > 0.0:
             raise ValueError("temperature must be > 0 for sampling modes")   # engine/sampling.py:75-76
         if self.mode is SamplingMode.TOP_P and not 0.0 < self.top_p <= 1.0:
             raise ValueError("top_p must be in (0, 1]")                      # engine/sampling.py:167-168
-        if self.repetition_penalty <= 0.0:
-            raise ValueError("repetition_penalty must be positive")
+        if self.mode is SamplingMode.TOP_K:
+            int(self.top_k)
+        operator.index(self.seed)
         if self.repetition_scope not in ("window", "history"):
             raise ValueError("repetition_scope must be 'window' or 'history'")
-        for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} must be finite")
-        for t, v in (self.logit_bias or {}).items():
+        if not self.repetition_penalty == 1.0 or not self.presence_penalty == 0.0 or not self.frequency_penalty == 0.0:
+            if self.repetition_penalty <= 0.0:
+                raise ValueError("repetition_penalty must be positive")
+            for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
+                if not math.isfinite(getattr(self, name)):
+                    raise ValueError(f"{name} must be finite")
+            if not 1e-37 <= self.repetition_penalty <= 1e38:
+                raise ValueError("repetition_penalty must be a float32 number: 1e-37 to 1e38")
+            if abs(self.presence_penalty) > 1e30 or abs(self.frequency_penalty) > 1e30:       # times a count it stays finite
+                raise ValueError("presence_penalty and frequency_penalty are 1e30 at most")
+        if not self.logit_bias:
+            return
+        if not isinstance(self.logit_bias, Mapping):
+            raise ValueError("logit_bias maps token ids to numbers")
+        for t, v in self.logit_bias.items():
             if isinstance(t, bool) or not isinstance(t, (int, np.integer)) or t < 0:
                 raise ValueError(f"logit_bias maps token ids to numbers, not {t!r}")
             if not math.isfinite(v) or abs(v) > 1e30:
@@ -114,15 +135,16 @@ def pack_rows(configs: list[SamplingConfig], keys: list[int], vocab: int) -> np.
     rows = np.zeros((m, 7), dtype=np.int32)
     f = rows.view(np.float32)
     u = rows.view(np.uint32)
-    for i, c in enumerate(configs):
+    for c in {id(c): c for c in configs}.values():       # rows of one configuration ask once
         c.validate()
+    for i, c in enumerate(configs):
         if c.mode is SamplingMode.GREEDY:
             f[i, 0], f[i, 1], rows[i, 2] = 0.0, 1.0, 0
         else:
             f[i, 0] = c.temperature
             f[i, 1] = c.top_p if c.mode is SamplingMode.TOP_P else 1.0
             rows[i, 2] = max(1, min(int(c.top_k), vocab)) if c.mode is SamplingMode.TOP_K else 0
-        seed, key = c.seed & _MASK64, keys[i] & _MASK64
+        seed, key = operator.index(c.seed) & _MASK64, keys[i] & _MASK64
         u[i, 3], u[i, 4] = seed & 0xFFFFFFFF, seed >> 32
         u[i, 5], u[i, 6] = key & 0xFFFFFFFF, key >> 32
     return rows
