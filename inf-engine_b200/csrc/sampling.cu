@@ -216,7 +216,8 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ x, const Sa
       above = block_sum(above, red);
       if (above < budget) K = cand;
     }
-    below = max(below, max(K, 1u) - 1u);      // the largest number is above it: the budget is more than nothing
+    below = max(below, max(K, 1u) - 1u);
+    below = min(below, order_key(m) - 1u);    // the largest stays, also where the budget is nothing in float32
   }
 
   // inverse CDF in vocabulary order over the kept tokens

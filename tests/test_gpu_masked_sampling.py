@@ -157,3 +157,14 @@ def test_a_temperature_that_divides_to_nothing_is_greedy(vocab):
     for mode in ("temperature", "top_k", "top_p"):
         got = draw(logits, [SamplingConfig(mode=mode, temperature=1e-40, seed=i) for i in range(8)], list(range(8)))
         assert torch.equal(got.long(), logits.argmax(1))
+
+
+@pytest.mark.parametrize("vocab", [100, 40003])
+@pytest.mark.parametrize("top_p", [1e-30, 1e-46])
+def test_the_largest_stays_under_the_smallest_top_p(vocab, top_p):
+    """1e-46 is 0 in float32, where no mass lies below the budget."""
+    from inf_engine_b200.sampling import SamplingConfig
+    logits = torch.randn(16, vocab, generator=torch.Generator().manual_seed(5))
+    for steps in (0, (1 << 24) - 1):
+        got = draw(logits, [SamplingConfig(mode="top_p", top_p=top_p, seed=seed_for(steps, k)) for k in range(16)], list(range(16)))
+        assert torch.equal(got.long(), logits.argmax(1))
