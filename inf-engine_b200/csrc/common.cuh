@@ -124,6 +124,11 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
 #define TANH_SMALL 0.5f
 #define TANH_COEFS 0.99999994f, -0.333327681f, 0.133204684f, -0.0527566522f, 0.0167278275f
 
+// Sizes that come as 64-bit words and go on as int: up to SIZE_MOST there is room above them for what kernels and launchers
+// round up to and step over.  True where one is larger, or negative.
+constexpr long long SIZE_MOST = 0x7f000000;
+template <typename... Sizes> static inline bool beyond(Sizes... sizes) { return (... || (sizes < 0 || sizes > SIZE_MOST)); }
+
 static inline int launch_status() { return (int)cudaGetLastError(); }
 
 // What has to be done once on every device, such as raising a kernel's limit of dynamic shared memory: a program may run

@@ -154,12 +154,12 @@ static int fp8_quantize_blocks(const void* w, int dtype, void* codes, float* sca
   return launch_k(quantize_blocks_kernel<bf16>, grid, BT, 0, stream, (const bf16*)w, (uint8_t*)codes, scales, rows, cols, ldw, ldc, vec);
 }
 
-// the entries: arguments as 64-bit words in the order above, which a caller converts in one go; sizes of 2^31 and more are refused
+// the entries: arguments as 64-bit words in the order above, which a caller converts in one go; sizes above SIZE_MOST are refused
 extern "C" int ie_fp8_quantize_rows(const long long* a) {
-  if ((a[4] | a[5]) >> 31) return IE_BAD_SIZE;
+  if (beyond(a[4], a[5])) return IE_BAD_SIZE;
   return fp8_quantize_rows((const void*)a[0], (int)a[1], (void*)a[2], (float*)a[3], (int)a[4], (int)a[5], a[6], a[7], a[8], a[9], (cudaStream_t)a[10]);
 }
 extern "C" int ie_fp8_quantize_blocks(const long long* a) {
-  if ((a[4] | a[5]) >> 31) return IE_BAD_SIZE;
+  if (beyond(a[4], a[5])) return IE_BAD_SIZE;
   return fp8_quantize_blocks((const void*)a[0], (int)a[1], (void*)a[2], (float*)a[3], (int)a[4], (int)a[5], a[6], a[7], (cudaStream_t)a[8]);
 }

@@ -1128,9 +1128,9 @@ static int gemm_fp8(const void* x, int x_dtype, const float* sx, const void* w, 
   return p.split > 1 ? launch_tiles<false, true>(p, sms, stream) : launch_tiles<false, false>(p, sms, stream);
 }
 
-// the entry: arguments as 64-bit words in the order above, which a caller converts in one go; sizes of 2^31 and more are refused
+// the entry: arguments as 64-bit words in the order above, which a caller converts in one go; sizes above SIZE_MOST are refused
 extern "C" int ie_gemm_fp8(const long long* a) {
-  if ((a[7] | a[8] | a[9]) >> 31) return IE_BAD_SIZE;
+  if (beyond(a[7], a[8], a[9])) return IE_BAD_SIZE;
   return gemm_fp8((const void*)a[0], (int)a[1], (const float*)a[2], (const void*)a[3], (const float*)a[4], (void*)a[5], (int)a[6], (int)a[7],
                   (int)a[8], (int)a[9], a[10], a[11], a[12], a[13], a[14], (void*)a[15], a[16], (cudaStream_t)a[17]);
 }

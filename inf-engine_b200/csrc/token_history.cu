@@ -259,18 +259,18 @@ static int adjust_logits(const void* logits, int dtype, float* out, const int* s
   return vec ? launch_k(adjust_logits_kernel<bf16, 4>, grid, HT, 0, stream, p) : launch_k(adjust_logits_kernel<bf16, 1>, grid, HT, 0, stream, p);
 }
 
-// the entries: arguments as 64-bit words in the order above, which a caller converts in one go; sizes of 2^31 and more are refused
+// the entries: arguments as 64-bit words in the order above, which a caller converts in one go; sizes above SIZE_MOST are refused
 extern "C" int ie_history_reset(const long long* a) {
-  if ((a[3] | a[4] | a[5]) >> 31) return IE_BAD_SIZE;
+  if (beyond(a[3], a[4], a[5])) return IE_BAD_SIZE;
   return history_reset((int*)a[0], (int*)a[1], (const int*)a[2], (int)a[3], (int)a[4], (int)a[5], (cudaStream_t)a[6]);
 }
 extern "C" int ie_history_append(const long long* a) {
-  if ((a[6] | a[7] | a[8] | a[9]) >> 31) return IE_BAD_SIZE;
+  if (beyond(a[6], a[7], a[8], a[9])) return IE_BAD_SIZE;
   return history_append((int*)a[0], (int*)a[1], (const int*)a[2], (const int*)a[3], (const int*)a[4], (const int*)a[5], (int)a[6],
                         (int)a[7], (int)a[8], (int)a[9], (cudaStream_t)a[10]);
 }
 extern "C" int ie_adjust_logits(const long long* a) {
-  if ((a[12] | a[13] | a[16] | a[17] | a[18]) >> 31) return IE_BAD_SIZE;
+  if (beyond(a[12], a[13], a[16], a[17], a[18])) return IE_BAD_SIZE;
   return adjust_logits((const void*)a[0], (int)a[1], (float*)a[2], (const int*)a[3], (const float*)a[4], (const int*)a[5],
                        (const int*)a[6], (const int*)a[7], (const int*)a[8], (const float*)a[9], (const int*)a[10], (const int*)a[11],
                        (int)a[12], (int)a[13], a[14], a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19], (cudaStream_t)a[20]);
