@@ -17,6 +17,7 @@
 #define IE_BAD_DTYPE -1
 #define IE_BAD_SIZE -2
 #define IE_BAD_ALIGN -3
+#define IE_OVERLAP -6      /* memory that is written lies over other arguments */
 
 // dtype codes used across the C interface
 #define IE_F32 0
@@ -128,6 +129,23 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
 // round up to and step over.  True where one is larger, or negative.
 constexpr long long SIZE_MOST = 0x7f000000;
 template <typename... Sizes> static inline bool beyond(Sizes... sizes) { return (... || (sizes < 0 || sizes > SIZE_MOST)); }
+
+// Memory of a matrix: `rows` stretches of `width` bytes, `pitch` bytes apart.
+struct Span {
+  uintptr_t at;
+  long long rows, width, pitch;
+};
+// Whether two of them share a byte; columns of one buffer, side by side, do not.
+static inline bool overlap(const Span& a, const Span& b) {
+  if (a.at == 0 || b.at == 0 || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  if (a.at + (a.rows - 1) * a.pitch + a.width <= b.at || b.at + (b.rows - 1) * b.pitch + b.width <= a.at) return false;
+  if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+  const long long pitch = a.rows > 1 ? a.pitch : b.pitch;
+  if (pitch <= 0) return true;
+  long long d = (long long)(b.at - a.at) % pitch;
+  if (d < 0) d += pitch;
+  return d < a.width || pitch - d < b.width;
+}
 
 static inline int launch_status() { return (int)cudaGetLastError(); }
 

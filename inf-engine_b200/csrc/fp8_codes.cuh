@@ -115,4 +115,10 @@ template <typename T> __device__ __forceinline__ uint2 codes8(const Raw8<T>& r, 
   return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
+// Memory of scales [rows, groups], float32: the larger stride goes from stretch to stretch.
+inline Span scales_span(const void* at, long long rows, long long groups, long long s_row, long long s_col) {
+  if (rows > 1 && (groups == 1 || s_row >= s_col)) return {(uintptr_t)at, rows, 4 * ((groups - 1) * s_col + 1), 4 * s_row};
+  return {(uintptr_t)at, groups, 4 * ((rows - 1) * s_row + 1), 4 * s_col};
+}
+
 }  // namespace

@@ -157,9 +157,15 @@ static int fp8_quantize_blocks(const void* w, int dtype, void* codes, float* sca
 // the entries: arguments as 64-bit words in the order above, which a caller converts in one go; sizes above SIZE_MOST are refused
 extern "C" int ie_fp8_quantize_rows(const long long* a) {
   if (beyond(a[4], a[5])) return IE_BAD_SIZE;
+  const long long groups = (a[5] + GROUP - 1) / GROUP, size = a[1] == IE_F32 ? 4 : 2;
+  const Span scales = scales_span((const void*)a[3], a[4], groups, a[8], a[9]);
+  if (overlap(scales, {(uintptr_t)a[2], a[4], a[5], a[7]}) || overlap(scales, {(uintptr_t)a[0], a[4], size * a[5], size * a[6]})) return IE_OVERLAP;
   return fp8_quantize_rows((const void*)a[0], (int)a[1], (void*)a[2], (float*)a[3], (int)a[4], (int)a[5], a[6], a[7], a[8], a[9], (cudaStream_t)a[10]);
 }
 extern "C" int ie_fp8_quantize_blocks(const long long* a) {
   if (beyond(a[4], a[5])) return IE_BAD_SIZE;
+  const long long groups = (a[5] + GROUP - 1) / GROUP, size = a[1] == IE_F32 ? 4 : 2;
+  const Span scales = scales_span((const void*)a[3], (a[4] + GROUP - 1) / GROUP, groups, groups, 1);
+  if (overlap(scales, {(uintptr_t)a[2], a[4], a[5], a[7]}) || overlap(scales, {(uintptr_t)a[0], a[4], size * a[5], size * a[6]})) return IE_OVERLAP;
   return fp8_quantize_blocks((const void*)a[0], (int)a[1], (void*)a[2], (float*)a[3], (int)a[4], (int)a[5], a[6], a[7], (cudaStream_t)a[8]);
 }

@@ -1131,6 +1131,12 @@ static int gemm_fp8(const void* x, int x_dtype, const float* sx, const void* w, 
 // the entry: arguments as 64-bit words in the order above, which a caller converts in one go; sizes above SIZE_MOST are refused
 extern "C" int ie_gemm_fp8(const long long* a) {
   if (beyond(a[7], a[8], a[9])) return IE_BAD_SIZE;
+  // out and scratch over the scales (the caller has compared them with x, w and each other)
+  const long long M = a[7], N = a[8], k_blocks = (a[9] + GROUP - 1) / GROUP, size = a[6] == IE_F32 ? 4 : 2;
+  const Span out = {(uintptr_t)a[5], M, size * N, size * a[14]}, scratch = {(uintptr_t)a[15], 1, a[16], a[16]};
+  const Span sw = scales_span((const void*)a[4], (N + GROUP - 1) / GROUP, k_blocks, k_blocks, 1);
+  const Span sx = scales_span((const void*)a[2], M, k_blocks, a[11], a[12]);
+  if (overlap(out, sw) || overlap(out, sx) || overlap(scratch, sw) || overlap(scratch, sx)) return IE_OVERLAP;
   return gemm_fp8((const void*)a[0], (int)a[1], (const float*)a[2], (const void*)a[3], (const float*)a[4], (void*)a[5], (int)a[6], (int)a[7],
                   (int)a[8], (int)a[9], a[10], a[11], a[12], a[13], a[14], (void*)a[15], a[16], (cudaStream_t)a[17]);
 }

@@ -18,7 +18,7 @@ from .csrc.build import load_library
 IE_F32, IE_BF16 = 0, 1
 _CODES = {torch.float32: IE_F32, torch.bfloat16: IE_BF16}
 _ERRORS = {-1: "unsupported dtype combination", -2: "unsupported size", -3: "misaligned pointer or stride",
-           -4: "size beyond the kernel's static limit"}
+           -4: "size beyond the kernel's static limit", -6: "memory that is written is shared with another argument"}
 
 
 class KernelError(RuntimeError):
