@@ -16,6 +16,7 @@
 // 8,191 (every other row starts between two words) 32.8; in float32, by pairs where a row starts on one, 36.9 and 43.0; number by
 // number 38.9 in bfloat16, 49.2 in float32.
 #include "fp8_codes.cuh"
+#include <numeric>
 
 namespace {
 
@@ -112,6 +113,15 @@ __global__ void __launch_bounds__(BT) quantize_blocks_kernel(const T* __restrict
   if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = exp2i(e);
 }
 
+#define IE_COINCIDE -7      /* two elements of the scales have one place */
+// Whether two elements of [rows, groups] have one place: i s_row = j s_col has its least solution at i = s_col / g, j = s_row / g.
+inline bool coincide(long long rows, long long groups, long long s_row, long long s_col) {
+  if ((rows > 1 && s_row == 0) || (groups > 1 && s_col == 0)) return rows > 0 && groups > 0;
+  if (rows < 2 || groups < 2) return false;
+  const long long g = std::gcd(s_row, s_col);
+  return s_col / g < rows && s_row / g < groups;
+}
+
 // whether rows of x can be read 16 bytes at a time
 inline int reads_vectors(const void* x, long long ld, int dtype) {
   return ((uintptr_t)x & 15) == 0 && ld % (dtype == IE_F32 ? 4 : 8) == 0;
@@ -160,6 +170,7 @@ extern "C" int ie_fp8_quantize_rows(const long long* a) {
   const long long groups = (a[5] + GROUP - 1) / GROUP, size = a[1] == IE_F32 ? 4 : 2;
   const Span scales = scales_span((const void*)a[3], a[4], groups, a[8], a[9]);
   if (overlap(scales, {(uintptr_t)a[2], a[4], a[5], a[7]}) || overlap(scales, {(uintptr_t)a[0], a[4], size * a[5], size * a[6]})) return IE_OVERLAP;
+  if (coincide(a[4], groups, a[8], a[9])) return IE_COINCIDE;
   return fp8_quantize_rows((const void*)a[0], (int)a[1], (void*)a[2], (float*)a[3], (int)a[4], (int)a[5], a[6], a[7], a[8], a[9], (cudaStream_t)a[10]);
 }
 extern "C" int ie_fp8_quantize_blocks(const long long* a) {

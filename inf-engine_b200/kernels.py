@@ -18,7 +18,8 @@ from .csrc.build import load_library
 IE_F32, IE_BF16 = 0, 1
 _CODES = {torch.float32: IE_F32, torch.bfloat16: IE_BF16}
 _ERRORS = {-1: "unsupported dtype combination", -2: "unsupported size", -3: "misaligned pointer or stride",
-           -4: "size beyond the kernel's static limit", -6: "memory that is written is shared with another argument"}
+           -4: "size beyond the kernel's static limit", -6: "memory that is written is shared with another argument",
+           -7: "elements of an output share a place"}
 
 
 class KernelError(RuntimeError):
@@ -1883,7 +1884,8 @@ def _rows_in(what: str, name: str, t: torch.Tensor) -> tuple[int, int]:
 
 def fp8_quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
     """x (float32 or bfloat16 [n, k]) as 8-bit floating point with a scale for each row and 128 columns:
-    ``codes`` (float8_e4m3fn [n, k], rows a multiple of 16 bytes apart) times ``scales`` (float32 [n, ceil(k / 128)], any strides).
+    ``codes`` (float8_e4m3fn [n, k], rows a multiple of 16 bytes apart) times ``scales`` (float32 [n, ceil(k / 128)], any strides that
+    give each its place).
     A scale is the least power of two that brings the group's largest finite number to at most 448 (1 for zeros); a code is
     the nearest e4m3 number to x / scale, ties to even, NaN for a number that is not finite.  The three share no memory."""
     what = "fp8_quantize_rows"

@@ -89,6 +89,20 @@ for case in range(1000):
 assert min(seen.values()) > 150, seen
 """
 
+PLACES = PRELUDE + """
+rng = random.Random(3)
+seen = {True: 0, False: 0}
+for case in range(3000):
+    rows, groups, s_row, s_col = rng.randint(1, 7), rng.randint(1, 7), rng.randint(0, 9), rng.randint(0, 9)
+    places = [i * s_row + j * s_col for i in range(rows) for j in range(groups)]
+    shared = len(set(places)) < len(places)
+    cols = 128 * groups - rng.randint(0, 127)
+    rc = fp8.ie_fp8_quantize_rows(kernels._11_words(A, 1, A + (1 << 20), A + (1 << 22), rows, cols, cols, 1024, s_row, s_col, 0))
+    assert (rc == -7) == shared, (case, rows, groups, s_row, s_col)
+    seen[shared] += 1
+assert min(seen.values()) > 500, seen
+"""
+
 
 def run(program):
     root = Path(__file__).resolve().parent.parent
@@ -103,6 +117,10 @@ def test_scales_of_the_quantisers():
 
 def test_scales_of_the_product():
     run(PRODUCT)
+
+
+def test_each_scale_has_its_place():
+    run(PLACES)
 
 
 @pytest.mark.gpu
@@ -133,3 +151,16 @@ def test_scales_beside_their_codes_and_over_them(n):
     room = torch.empty(8192, dtype=torch.uint8, device="cuda")
     with pytest.raises(kernels.KernelError, match="shared with another argument"):
         kernels.gemm_fp8(x, w, room[-24:].view(torch.float32).view(2, 3), out[:n * 130].view(n, 130), scratch=room)
+
+
+@pytest.mark.gpu
+def test_expanded_scales_are_refused_as_an_output():
+    from inf_engine_b200 import kernels
+    from test_gpu_fp8 import codes_of, rows
+    x = rows(4, 300, torch.bfloat16, 1)
+    codes, one = kernels.fp8_empty(4, 300, "cuda"), torch.zeros(1, 3, device="cuda")
+    with pytest.raises(kernels.KernelError, match="share a place"):
+        kernels.fp8_quantize_rows(x, codes, one.expand(4, 3))
+    woven = torch.zeros(64, device="cuda").as_strided((4, 3), (2, 9))          # odd, but each has its own
+    kernels.fp8_quantize_rows(x, codes, woven)
+    assert torch.equal(woven.double(), codes_of(x)[1])
