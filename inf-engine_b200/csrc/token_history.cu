@@ -16,6 +16,7 @@
 // stores) and 196,000 tokens added to them 4.9 us; 64 rows of 128,256 logits adjusted 17.9 us with 8,000 tokens seen, 100 biases and
 // a mask on every second row, 11.5 as a copy (5.7 TB/s).
 #include "common.cuh"
+#include <initializer_list>
 
 namespace {
 
@@ -259,18 +260,35 @@ static int adjust_logits(const void* logits, int dtype, float* out, const int* s
   return vec ? launch_k(adjust_logits_kernel<bf16, 4>, grid, HT, 0, stream, p) : launch_k(adjust_logits_kernel<bf16, 1>, grid, HT, 0, stream, p);
 }
 
+// vectors and tables of words (of the logits: rows of them) that a call reads, or writes
+static Span words(long long at, long long n) { return {(uintptr_t)at, 1, 4 * n, 4 * n}; }
+static bool any_overlap(const Span& written, std::initializer_list<Span> others) {
+  for (const Span& o : others)
+    if (overlap(written, o)) return true;
+  return false;
+}
+
 // the entries: arguments as 64-bit words in the order above, which a caller converts in one go; sizes above SIZE_MOST are refused
 extern "C" int ie_history_reset(const long long* a) {
   if (beyond(a[3], a[4], a[5])) return IE_BAD_SIZE;
+  const Span counts = words(a[0], a[4] * a[5]), seen = words(a[1], a[4] * ((a[5] + 31) / 32)), slots = words(a[2], a[3]);
+  if (any_overlap(counts, {seen, slots}) || overlap(seen, slots)) return IE_OVERLAP;
   return history_reset((int*)a[0], (int*)a[1], (const int*)a[2], (int)a[3], (int)a[4], (int)a[5], (cudaStream_t)a[6]);
 }
 extern "C" int ie_history_append(const long long* a) {
   if (beyond(a[6], a[7], a[8], a[9])) return IE_BAD_SIZE;
+  const Span counts = words(a[0], a[8] * a[9]), seen = words(a[1], a[8] * ((a[9] + 31) / 32));
+  const Span tokens = words(a[2], a[6]), slots = words(a[3], a[7]), starts = words(a[4], a[7] + 1), n_prompt = words(a[5], a[7]);
+  if (any_overlap(counts, {seen, tokens, slots, starts, n_prompt}) || any_overlap(seen, {tokens, slots, starts, n_prompt})) return IE_OVERLAP;
   return history_append((int*)a[0], (int*)a[1], (const int*)a[2], (const int*)a[3], (const int*)a[4], (const int*)a[5], (int)a[6],
                         (int)a[7], (int)a[8], (int)a[9], (cudaStream_t)a[10]);
 }
 extern "C" int ie_adjust_logits(const long long* a) {
   if (beyond(a[12], a[13], a[16], a[17], a[18])) return IE_BAD_SIZE;
+  const long long rows = a[12], vocab = a[13], bits = (vocab + 31) / 32;      // out against logits is the caller's, who knows whether they are one
+  const Span out = {(uintptr_t)a[2], rows, 4 * vocab, 4 * a[15]};
+  if (any_overlap(out, {words(a[3], rows), words(a[4], 3 * rows), words(a[5], a[16] * vocab), words(a[6], a[16] * bits), words(a[7], rows + 1),
+                        words(a[8], a[17]), words(a[9], a[17]), words(a[10], rows), words(a[11], a[18] * bits)})) return IE_OVERLAP;
   return adjust_logits((const void*)a[0], (int)a[1], (float*)a[2], (const int*)a[3], (const float*)a[4], (const int*)a[5],
                        (const int*)a[6], (const int*)a[7], (const int*)a[8], (const float*)a[9], (const int*)a[10], (const int*)a[11],
                        (int)a[12], (int)a[13], a[14], a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19], (cudaStream_t)a[20]);

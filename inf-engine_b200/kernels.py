@@ -1126,7 +1126,7 @@ def _history(what: str, counts: torch.Tensor, seen: torch.Tensor) -> tuple[int, 
 def history_reset(counts: torch.Tensor, seen: torch.Tensor, slots: torch.Tensor) -> None:
     """Forgets what the requests in ``slots`` (int32 [n]) have said: counts[slot] = 0, seen[slot] = 0.  A slot that is
     negative, or beyond the table, is passed over.  ``counts`` int32 [slots, vocab]; ``seen`` int32 [slots, ceil(vocab / 32)],
-    bit t % 32 of word t / 32."""
+    bit t % 32 of word t / 32; the three share no memory."""
     n_slots, vocab = _history("history_reset", counts, seen)
     if slots.dim() != 1 or slots.dtype is not _I32 or not slots.is_contiguous():
         _refuse("history_reset", "slots is a contiguous int32 [n]")
@@ -1142,7 +1142,8 @@ def history_append(counts: torch.Tensor, seen: torch.Tensor, tokens: torch.Tenso
     """Adds ``tokens`` (int32 [T]) to the histories of ``slots`` (int32 [R]).  Tokens ``starts[r] .. starts[r + 1]`` (int32 [R + 1],
     ascending; None: one token a slot) belong to slot r, and the first ``n_prompt[r]`` of them (int32 [R]; None: none) to its prompt:
     those set the bit in ``seen``; every other token also adds one to ``counts``.  A token outside the vocabulary, or of a slot that
-    is negative or beyond the table, is passed over.  Tokens and slots may come more than once."""
+    is negative or beyond the table, is passed over.  Tokens and slots may come more than once.  ``counts`` and ``seen`` share no memory with
+    each other or with what is read."""
     what = "history_append"
     n_slots, vocab = _history(what, counts, seen)
     if (tokens.dim() != 1 or tokens.dtype is not _I32 or not tokens.is_contiguous() or slots.dim() != 1 or slots.dtype is not _I32
@@ -1193,7 +1194,7 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, slots: torch.Tensor |
                   bias_values: torch.Tensor | None = None, mask_rows: torch.Tensor | None = None,
                   masks: torch.Tensor | None = None) -> None:
     """out = logits (float32 or bfloat16 [n, vocab]) with each row's penalties, biases and mask, float32.  ``out`` may be ``logits``
-    itself; otherwise the two share no memory.
+    itself; otherwise the two share no memory, and ``out`` shares none with the tables below.
 
     Penalties (all four or none): row i reads the history ``slots[i]`` (int32 [n]; outside the table: none) and
     ``penalties[i]`` = (repetition, presence, frequency), float32 [n, 3].  The logit of a token that is in ``seen`` is divided

@@ -103,6 +103,47 @@ for case in range(3000):
 assert min(seen.values()) > 500, seen
 """
 
+TABLES = PRELUDE + """
+# every argument has its own place, and every one that is written is then moved over every other one's first and last word
+def check(call, pack, layout, words, written):
+    # layout: name -> (index of the address, number of words); words: the arguments, addresses included
+    at = {}
+    place = A
+    for name, (i, n) in layout.items():
+        at[name] = words[i] = place
+        place += 4 * n
+    assert call(pack(*words)) != OVERLAP
+    for w in written:
+        for name, (i, n) in layout.items():
+            if name == w:
+                continue
+            iw, nw = layout[w]
+            for moved, refused in ((at[name] - 4 * nw, False), (at[name] - 4 * nw + 4, True), (at[name] + 4 * n - 4, True), (at[name] + 4 * n, False)):
+                other = list(words)
+                for j, (k, _) in enumerate(layout.values()):
+                    if k != i:
+                        other[k] = A * 100 + (j << 30)        # the others far away
+                other[iw] = moved
+                rc = call(pack(*other))
+                assert (rc == OVERLAP) == refused, (call.__name__, w, name, moved - at[name])
+v, bits, slots, n, tokens, masks, biases = 1000, 32, 5, 3, 40, 4, 17
+check(core.ie_history_reset, kernels._7_words, {"counts": (0, slots * v), "seen": (1, slots * bits), "slots": (2, n)},
+      [0, 0, 0, n, slots, v, 0], ("counts", "seen"))
+check(core.ie_history_append, kernels._11_words,
+      {"counts": (0, slots * v), "seen": (1, slots * bits), "tokens": (2, tokens), "slots": (3, n), "starts": (4, n + 1), "n_prompt": (5, n)},
+      [0] * 6 + [tokens, n, slots, v, 0], ("counts", "seen"))
+layout = {"out": (2, n * v), "slots": (3, n), "penalties": (4, 3 * n), "counts": (5, slots * v), "seen": (6, slots * bits), "bias_start": (7, n + 1),
+          "bias_ids": (8, biases), "bias_values": (9, biases), "mask_rows": (10, n), "masks": (11, masks * bits)}
+check(core.ie_adjust_logits, kernels._21_words, layout, [A * 1000, 0] + [0] * 10 + [n, v, v, v, slots, biases, masks, 0, 0], ("out",))
+# a table between the rows of out
+words = [A * 1000, 0, A] + [0] * 9 + [n, v, v, v + 50, slots, biases, masks, 0, 0]
+for gap, refused in ((0, False), (18, False), (19, True), (-1, True)):
+    words[11] = A + 4 * (v + gap)                           # 32 words of one mask in a gap of 50
+    words[18] = 1
+    rc = core.ie_adjust_logits(kernels._21_words(*words))
+    assert (rc == OVERLAP) == refused, gap
+"""
+
 
 def run(program):
     root = Path(__file__).resolve().parent.parent
@@ -121,6 +162,10 @@ def test_scales_of_the_product():
 
 def test_each_scale_has_its_place():
     run(PLACES)
+
+
+def test_tables_of_histories_and_logits():
+    run(TABLES)
 
 
 @pytest.mark.gpu
@@ -164,3 +209,21 @@ def test_expanded_scales_are_refused_as_an_output():
     woven = torch.zeros(64, device="cuda").as_strided((4, 3), (2, 9))          # odd, but each has its own
     kernels.fp8_quantize_rows(x, codes, woven)
     assert torch.equal(woven.double(), codes_of(x)[1])
+
+
+@pytest.mark.gpu
+def test_tables_over_what_is_written_are_refused():
+    from inf_engine_b200 import kernels
+    i32 = dict(dtype=torch.int32, device="cuda")
+    counts, seen = torch.zeros(3, 64, **i32), torch.zeros(3, 2, **i32)
+    one = torch.zeros(1, **i32)
+    for call in (lambda: kernels.history_reset(counts, counts.view(-1)[:6].view(3, 2), one), lambda: kernels.history_reset(counts, seen, seen[1, :1]),
+                 lambda: kernels.history_append(counts, seen, counts[0, :1], one), lambda: kernels.history_append(counts, seen, one, seen[2, 1:])):
+        with pytest.raises(kernels.KernelError, match="shared with another argument"):
+            call()
+    logits = torch.zeros(3, 64, device="cuda")
+    with pytest.raises(kernels.KernelError, match="shared with another argument"):
+        kernels.adjust_logits(logits, logits, mask_rows=torch.zeros(3, **i32), masks=logits.view(torch.int32)[:1, :2])
+    kernels.history_append(counts, seen, one, one)
+    kernels.history_reset(counts, seen, one)
+    assert not bool(counts.any()) and not bool(seen.any())
