@@ -56,10 +56,6 @@ class ModelRunner:
         torch.cuda.set_device(self.device)
         self.rt = Runtime(self.device, self.dtype, weights)
         self.model = build_model(self.spec, tensors, self.rt)     # the top level that spec.kind names
-        if weights:
-            for layer in getattr(self.model, "layers", ()):
-                if getattr(layer.mixer, "o_weight", None) is not None:
-                    layer.mixer.o_weight = None                   # its product holds the codes
         max_pages_per_request = -(-self.spec.max_positions // page_size)
         self.cache = CacheManager(self.model.cache_requirements(), page_size, n_pages, max_requests,
                                   min(n_pages, max_pages_per_request))

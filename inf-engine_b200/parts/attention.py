@@ -93,8 +93,8 @@ class PagedAttention:
         ws = [tensors[spec.q_proj], tensors[spec.k_proj], tensors[spec.v_proj]]
         dtype = torch.float32 if any(w.dtype is torch.float32 for w in ws) else ws[0].dtype
         self.qkv = Linear(torch.cat([w.to(dtype) for w in ws], dim=0).contiguous(), rt, "qkv")
-        self.o_weight = tensors[spec.o_proj]
-        self.o = Linear(self.o_weight, rt, "o")
+        self.o = Linear(tensors[spec.o_proj], rt, "o")
+        self.o_weight = None if self.o.scales is not None else tensors[spec.o_proj]       # as it came; codes stand for it alone
         self.position = build_position(spec.position, tensors, rt)
         self.scale = float(spec.scale) if spec.scale is not None else float(spec.head_dim) ** -0.5
         self.v_dim = spec.value_dim

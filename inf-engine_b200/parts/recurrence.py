@@ -70,8 +70,8 @@ class GatedLinearRecurrence:
         self.a_gate, self.i_gate = tensors[spec.a_gate].contiguous(), tensors[spec.i_gate].contiguous()
         self.a_bias, self.i_bias, self.lam = same_dtype([tensors[spec.a_gate_bias].reshape(-1),
                                                          tensors[spec.i_gate_bias].reshape(-1), tensors[spec.lam]])
-        self.o_weight = tensors[spec.o_proj]
-        self.o = Linear(self.o_weight, rt, "o")
+        self.o = Linear(tensors[spec.o_proj], rt, "o")
+        self.o_weight = None if self.o.scales is not None else tensors[spec.o_proj]       # as it came; codes stand for it alone
         self.core_width = spec.width
 
     def cache_requirement(self) -> CacheRequirement:
@@ -164,7 +164,7 @@ class ParallelMixer:
         # one output product for all branches when each can say what goes into its own
         self.joint = all(hasattr(b, "forward_core") and hasattr(b, "o_weight") for b in self.branches)
         if self.joint:
-            ws = [b.o_weight for b in self.branches]
+            ws = [tensors[b.o_proj] for b in spec.branches]
             dtype = torch.float32 if any(w.dtype is torch.float32 for w in ws) else ws[0].dtype
             self.o = Linear(torch.cat([w.to(dtype) for w in ws], dim=1).contiguous(), rt, "o")
             self.widths = [b.core_width for b in self.branches]
