@@ -70,7 +70,10 @@ def _parse_ids(text: str) -> list[list[int]]:
 def _parse_bias(text: str | None) -> dict[int, float] | None:
     if not text:
         return None
-    return {int(t): float(v) for t, v in (part.split(":") for part in text.split(",") if part)}
+    try:
+        return {int(t): float(v) for t, v in (part.split(":") for part in text.split(",") if part)}
+    except ValueError:
+        raise ValueError(f"--logit-bias is ID:NUMBER,ID:NUMBER,..., not {text!r}") from None
 
 
 def main(argv=None) -> int:
@@ -83,6 +86,15 @@ def main(argv=None) -> int:
     if args.list_presets:
         print("\n".join(preset_names()))
         return 0
+    try:
+        sampling = SamplingConfig(mode=args.mode, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
+                                  repetition_penalty=args.repetition_penalty, seed=args.seed, repetition_scope=args.repetition_scope,
+                                  presence_penalty=args.presence_penalty, frequency_penalty=args.frequency_penalty,
+                                  logit_bias=_parse_bias(args.logit_bias))
+        sampling.validate()
+    except ValueError as e:
+        print(e, file=sys.stderr)
+        return 2
     model_dir = args.model_dir or (args.model if args.model and Path(args.model).is_dir() else None)
     prompts: list[list[int]] = []
     tokenizer = None
@@ -123,10 +135,6 @@ def main(argv=None) -> int:
         print("give --model-dir DIR, or --model PRESET --random-weights", file=sys.stderr)
         return 2
     t_load = time.perf_counter() - t0
-    sampling = SamplingConfig(mode=args.mode, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
-                              repetition_penalty=args.repetition_penalty, seed=args.seed, repetition_scope=args.repetition_scope,
-                              presence_penalty=args.presence_penalty, frequency_penalty=args.frequency_penalty,
-                              logit_bias=_parse_bias(args.logit_bias))
     requests = [Request(req_id=i, prompt_ids=p, max_new_tokens=args.n, sampling=sampling) for i, p in enumerate(prompts)]
     t0 = time.perf_counter()
     out = engine.run_offline(requests)
