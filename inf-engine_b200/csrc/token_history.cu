@@ -14,7 +14,8 @@
 //
 // Measured (device): 64 tokens appended 1.9 us, a launch and three dependent loads; 64 slots of 128,256 cleared 6.6 us (5.3 TB/s of
 // stores) and 196,000 tokens added to them 4.9 us; 64 rows of 128,256 logits adjusted 17.9 us with 8,000 tokens seen, 100 biases and
-// a mask on every second row, 11.5 as a copy (5.7 TB/s).
+// a mask on every second row, 11.5 as a copy (5.7 TB/s).  Biases alone, in place: 64 rows with 100 each 7.0 us, with 1,000 22.7, one row
+// that names every token 0.57 ms (with a search through the row's list for each of its biases 11.1, 179 and 119 ms).
 #include "common.cuh"
 #include <initializer_list>
 
@@ -113,13 +114,16 @@ constexpr int ADJUST_STEPS = 4, ADJUST_TOKENS = 4096;
 
 template <typename T, int V>
 __global__ void __launch_bounds__(HT, 8) adjust_logits_kernel(AdjustParams p) {
-  __shared__ unsigned short list[ADJUST_TOKENS];       // tokens to penalise, from the block's first on, in no order that matters
+  __shared__ __align__(16) unsigned char shared[4 * ADJUST_TOKENS];
+  unsigned short* list = reinterpret_cast<unsigned short*>(shared);    // tokens to penalise, from the block's first on, in no order that matters
+  __shared__ unsigned named[ADJUST_TOKENS / 32];       // tokens that have biases
   __shared__ int listed;
   pdl_trigger();
+  const int row = blockIdx.y, lo = blockIdx.x * p.chunk, hi = min(p.vocab, lo + p.chunk);     // a chunk is whole words of bits
   if (threadIdx.x == 0) listed = 0;
+  if (threadIdx.x < ADJUST_TOKENS / 32) named[threadIdx.x] = 0u;
   __syncthreads();
   pdl_wait();
-  const int row = blockIdx.y, lo = blockIdx.x * p.chunk, hi = min(p.vocab, lo + p.chunk);     // a chunk is whole words of bits
   const T* x = (const T*)p.logits + row * p.ld_in;
   float* out = p.out + row * p.ld_out;
   int slot = p.slots != nullptr ? p.slots[row] : -1;
@@ -192,28 +196,44 @@ __global__ void __launch_bounds__(HT, 8) adjust_logits_kernel(AdjustParams p) {
   }
   if (p.bias_start == nullptr) return;
   const int b0 = max(0, p.bias_start[row]), b1 = min(p.n_bias, p.bias_start[row + 1]);
-  if (b0 >= b1) return;
-  __syncthreads();
-  // 32 biases a warp at a time; for each one that falls into this block's logits the whole warp looks through the row's list, for a
-  // token that comes twice: its first bias takes all of them, in order, and the later ones nothing
-  const int lane = threadIdx.x & 31;
-  for (int bw = b0 + (threadIdx.x & ~31); bw < b1; bw += HT) {
-    const int mine = bw + lane < b1 ? p.bias_ids[bw + lane] : -1;
-    const bool takes = mine >= lo && mine < hi && !(mask && !((mask[mine >> 5] >> (mine & 31)) & 1));
-    for (unsigned left = __ballot_sync(0xffffffffu, takes); left; left &= left - 1) {
-      const int at = bw + __ffs(left) - 1, t = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
-      bool earlier = false;
-      float sum = 0.f;
-      for (int j0 = b0; j0 < b1 && !earlier; j0 += 32) {
-        unsigned same = __ballot_sync(0xffffffffu, j0 + lane < b1 && p.bias_ids[j0 + lane] == t);
-        for (; same && !earlier; same &= same - 1) {
-          const int j = j0 + __ffs(same) - 1;
-          earlier = j < at;
-          sum += p.bias_values[j];
-        }
+  bool here = false;
+  for (int j = b0 + threadIdx.x; j < b1; j += HT) here |= p.bias_ids[j] >= lo && p.bias_ids[j] < hi;
+  if (!__syncthreads_or(here)) return;                 // the passes above are done in the whole block
+  // Every warp goes through the row's list and adds up those of an eighth of the tokens, in the list's order: the time is in
+  // proportion to the list, whatever it names and how often.  A sum that has not been begun is known by its bit.
+  float* sums = reinterpret_cast<float*>(shared);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int j0 = b0 + lane; j0 - lane < b1; j0 += 32 * ADJUST_STEPS) {
+    int ids[ADJUST_STEPS];
+#pragma unroll
+    for (int s = 0; s < ADJUST_STEPS; ++s) ids[s] = j0 + 32 * s < b1 ? p.bias_ids[j0 + 32 * s] : -1;
+#pragma unroll
+    for (int s = 0; s < ADJUST_STEPS; ++s) {
+      const int t = ids[s], at = t - lo;
+      const bool mine = t >= lo && t < hi && (t & 7) == warp && !(mask && !((mask[t >> 5] >> (t & 31)) & 1));
+      const unsigned some = __ballot_sync(0xffffffffu, mine);
+      if (some == 0) continue;
+      const float v = mine ? p.bias_values[j0 + 32 * s] : 0.f;
+      const unsigned same = __match_any_sync(0xffffffffu, mine ? t : ~lane);     // lanes of the same token
+      const bool first = mine && __ffs(same) - 1 == lane;
+      float sum = first && ((named[at >> 5] >> (at & 31)) & 1) ? sums[at] : 0.f;
+      for (unsigned left = some; left; left &= left - 1) {
+        const int k = __ffs(left) - 1;
+        const float vk = __shfl_sync(0xffffffffu, v, k);
+        if ((same >> k) & 1) sum += vk;
       }
-      if (!earlier && lane == 0) out[t] += sum;
+      if (first) {
+        sums[at] = sum;
+        atomicOr(&named[at >> 5], 1u << (at & 31));
+      }
+      __syncwarp();
     }
+  }
+  __syncthreads();
+  static_assert(ADJUST_TOKENS / 16 == HT, "a thread has the bits of 16 tokens");
+  for (unsigned bits = (named[threadIdx.x >> 1] >> (16 * (threadIdx.x & 1))) & 0xffffu; bits; bits &= bits - 1) {
+    const int at = 16 * threadIdx.x + __ffs(bits) - 1;
+    out[lo + at] += sums[at];
   }
 }
 
