@@ -14,8 +14,8 @@
 //
 // Measured (device): 64 tokens appended 1.9 us, a launch and three dependent loads; 64 slots of 128,256 cleared 6.6 us (5.3 TB/s of
 // stores) and 196,000 tokens added to them 4.9 us; 64 rows of 128,256 logits adjusted 17.9 us with 8,000 tokens seen, 100 biases and
-// a mask on every second row, 11.5 as a copy (5.7 TB/s).  Biases alone, in place: 64 rows with 100 each 7.0 us, with 1,000 22.7, one row
-// that names every token 0.57 ms (with a search through the row's list for each of its biases 11.1, 179 and 119 ms).
+// a mask on every second row, 11.5 as a copy (5.7 TB/s).  Biases alone, in place: 64 rows with 100 each 6.6 us, with 1,000 23.4, one row
+// that names every token 0.51 ms (with a search through the row's list for each of its biases 11.1, 179 and 119 ms).
 #include "common.cuh"
 #include <initializer_list>
 
@@ -112,6 +112,68 @@ struct AdjustParams {
 // longer than the memory does (64 rows of 128,256: 23 us against 12 so).  In place the first pass writes what is masked and no more.
 constexpr int ADJUST_STEPS = 4, ADJUST_TOKENS = 4096;
 
+// The biases of a block's tokens.  Every warp goes through the row's list and adds up those of an eighth of the tokens, in the list's order:
+// the time is in proportion to the list, whatever it names and how often.  A sum that has not been begun is known by its bit in `named`
+// (ADJUST_TOKENS of both).  Row, stretch and pointers are found again from the block's index, which passes for unknown: kept from the
+// passes before they cost those registers (spills, 1.4 us).
+__device__ __forceinline__ void add_biases(const AdjustParams& p, float* sums, unsigned* named) {
+  int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
+  asm volatile("" : "+r"(row), "+r"(chunk), "+r"(tid));
+  const int b0 = max(0, p.bias_start[row]), b1 = min(p.n_bias, p.bias_start[row + 1]);
+  const int lo = chunk * p.chunk, hi = min(p.vocab, lo + p.chunk);
+  const int mask_row = p.mask_rows != nullptr ? p.mask_rows[row] : -1;
+  const int* mask = mask_row >= 0 && mask_row < p.n_masks ? p.masks + (size_t)mask_row * p.words : nullptr;
+  const int* ids = p.bias_ids;
+  const float* values = p.bias_values;
+  float* out = p.out + row * p.ld_out;
+  const auto takes = [&](int t) { return t >= lo && t < hi && !(mask && !((mask[t >> 5] >> (t & 31)) & 1)); };
+  bool here = false;
+  for (int j = b0 + tid; j < b1; j += HT) here |= takes(ids[j]);
+  if (!__syncthreads_or(here)) return;                 // what was written before is there for the whole block
+  const int lane = tid & 31, warp = tid >> 5;
+  for (int j0 = b0 + lane; j0 - lane < b1; j0 += 32 * ADJUST_STEPS) {
+    int next[ADJUST_STEPS];
+#pragma unroll
+    for (int s = 0; s < ADJUST_STEPS; ++s) next[s] = j0 + 32 * s < b1 ? ids[j0 + 32 * s] : -1;
+#pragma unroll
+    for (int s = 0; s < ADJUST_STEPS; ++s) {
+      const int t = next[s], at = (int)((unsigned)t - (unsigned)lo);
+      const bool mine = (t & 7) == warp && takes(t);
+      const unsigned some = __ballot_sync(0xffffffffu, mine);
+      if (some == 0) continue;
+      if ((some & (some - 1)) == 0) {                  // one alone, as in a list that is short against the vocabulary
+        if (mine) {
+          const unsigned bit = 1u << (at & 31);
+          sums[at] = ((named[at >> 5] & bit) ? sums[at] : 0.f) + values[j0 + 32 * s];
+          atomicOr(&named[at >> 5], bit);
+        }
+        __syncwarp();
+        continue;
+      }
+      const float v = mine ? values[j0 + 32 * s] : 0.f;
+      const unsigned same = __match_any_sync(0xffffffffu, mine ? t : ~lane);     // lanes of the same token
+      const bool first = mine && __ffs(same) - 1 == lane;
+      float sum = first && ((named[at >> 5] >> (at & 31)) & 1) ? sums[at] : 0.f;
+      for (unsigned left = some; left; left &= left - 1) {
+        const int k = __ffs(left) - 1;
+        const float vk = __shfl_sync(0xffffffffu, v, k);
+        if ((same >> k) & 1) sum += vk;
+      }
+      if (first) {
+        sums[at] = sum;
+        atomicOr(&named[at >> 5], 1u << (at & 31));
+      }
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  static_assert(ADJUST_TOKENS / 16 == HT, "a thread has the bits of 16 tokens");
+  for (unsigned bits = (named[tid >> 1] >> (16 * (tid & 1))) & 0xffffu; bits; bits &= bits - 1) {
+    const int at = 16 * tid + __ffs(bits) - 1;
+    out[lo + at] += sums[at];
+  }
+}
+
 template <typename T, int V>
 __global__ void __launch_bounds__(HT, 8) adjust_logits_kernel(AdjustParams p) {
   __shared__ __align__(16) unsigned char shared[4 * ADJUST_TOKENS];
@@ -195,46 +257,7 @@ __global__ void __launch_bounds__(HT, 8) adjust_logits_kernel(AdjustParams p) {
     }
   }
   if (p.bias_start == nullptr) return;
-  const int b0 = max(0, p.bias_start[row]), b1 = min(p.n_bias, p.bias_start[row + 1]);
-  bool here = false;
-  for (int j = b0 + threadIdx.x; j < b1; j += HT) here |= p.bias_ids[j] >= lo && p.bias_ids[j] < hi;
-  if (!__syncthreads_or(here)) return;                 // the passes above are done in the whole block
-  // Every warp goes through the row's list and adds up those of an eighth of the tokens, in the list's order: the time is in
-  // proportion to the list, whatever it names and how often.  A sum that has not been begun is known by its bit.
-  float* sums = reinterpret_cast<float*>(shared);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int j0 = b0 + lane; j0 - lane < b1; j0 += 32 * ADJUST_STEPS) {
-    int ids[ADJUST_STEPS];
-#pragma unroll
-    for (int s = 0; s < ADJUST_STEPS; ++s) ids[s] = j0 + 32 * s < b1 ? p.bias_ids[j0 + 32 * s] : -1;
-#pragma unroll
-    for (int s = 0; s < ADJUST_STEPS; ++s) {
-      const int t = ids[s], at = t - lo;
-      const bool mine = t >= lo && t < hi && (t & 7) == warp && !(mask && !((mask[t >> 5] >> (t & 31)) & 1));
-      const unsigned some = __ballot_sync(0xffffffffu, mine);
-      if (some == 0) continue;
-      const float v = mine ? p.bias_values[j0 + 32 * s] : 0.f;
-      const unsigned same = __match_any_sync(0xffffffffu, mine ? t : ~lane);     // lanes of the same token
-      const bool first = mine && __ffs(same) - 1 == lane;
-      float sum = first && ((named[at >> 5] >> (at & 31)) & 1) ? sums[at] : 0.f;
-      for (unsigned left = some; left; left &= left - 1) {
-        const int k = __ffs(left) - 1;
-        const float vk = __shfl_sync(0xffffffffu, v, k);
-        if ((same >> k) & 1) sum += vk;
-      }
-      if (first) {
-        sums[at] = sum;
-        atomicOr(&named[at >> 5], 1u << (at & 31));
-      }
-      __syncwarp();
-    }
-  }
-  __syncthreads();
-  static_assert(ADJUST_TOKENS / 16 == HT, "a thread has the bits of 16 tokens");
-  for (unsigned bits = (named[threadIdx.x >> 1] >> (16 * (threadIdx.x & 1))) & 0xffffu; bits; bits &= bits - 1) {
-    const int at = 16 * threadIdx.x + __ffs(bits) - 1;
-    out[lo + at] += sums[at];
-  }
+  add_biases(p, reinterpret_cast<float*>(shared), named);
 }
 
 }  // namespace
