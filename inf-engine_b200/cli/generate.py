@@ -44,7 +44,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--seed", type=int, default=0, help="sampling seed")
     p.add_argument("--dtype", choices=["bfloat16", "float32", "bf16", "fp32"], default="bfloat16")
     p.add_argument("--weights", choices=["fp8"], default=None,
-                   help="keep the layers' matrices in 8-bit floating point (with --dtype bfloat16)")
+                   help="keep the layers' matrices in 8-bit floating point (with --dtype bfloat16): less memory, slower steps of "
+                        "few requests")
     p.add_argument("--device", default="cuda:0")
     p.add_argument("--max-ctx", type=int, default=None, help="size the cache pool for this many tokens")
     p.add_argument("--n-total-blocks", type=int, default=None, help="pages in the cache pool")

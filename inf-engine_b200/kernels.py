@@ -1859,7 +1859,7 @@ def fp8_empty(rows: int, cols: int, device) -> torch.Tensor:
     return torch.empty((rows, max(16, -(-cols // 16) * 16)), dtype=FP8, device=device)[:, :cols]
 
 
-def _codes(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
+def _code_rows(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
     """(rows, columns, bytes from row to row) of a matrix of codes."""
     if t.dim() != 2 or t.dtype is not FP8:
         _refuse(what, f"{name} is a float8_e4m3fn matrix")
@@ -1891,7 +1891,7 @@ def fp8_quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
     the nearest e4m3 number to x / scale, ties to even, NaN for a number that is not finite.  The three share no memory."""
     what = "fp8_quantize_rows"
     code, ldx = _rows_in(what, "x", x)
-    n, k, pitch = _codes(what, "codes", codes)
+    n, k, pitch = _code_rows(what, "codes", codes)
     if x.shape != (n, k):
         _refuse(what, "codes has another shape than x")
     if scales.shape != (n, (k + 127) // 128) or scales.dtype is not _F32:
@@ -1912,7 +1912,7 @@ def fp8_quantize_blocks(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     [ceil(n / 128), ceil(k / 128)]."""
     what = "fp8_quantize_blocks"
     code, ldw = _rows_in(what, "w", w)
-    n, k, pitch = _codes(what, "codes", codes)
+    n, k, pitch = _code_rows(what, "codes", codes)
     if w.shape != (n, k):
         _refuse(what, "codes has another shape than w")
     if scales.shape != ((n + 127) // 128, (k + 127) // 128) or scales.dtype is not _F32 or not scales.is_contiguous():
@@ -1938,10 +1938,11 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
     [ceil(n / 128), ceil(k / 128)], any positive numbers); ``x`` codes with ``x_scales`` (float32 [m, ceil(k / 128)], any strides), or
     float32 / bfloat16 rows, which are quantised as ``fp8_quantize_rows`` does.  Codes lie as ``fp8_empty`` lays them out.  Sums are
     float32: inside a block of 128 columns on the tensor cores, over the scaled blocks in registers.  ``out`` shares no memory with
-    the operands.  ``scratch`` (uint8, at least ``gemm_fp8_scratch_bytes(x)``) takes the codes of rows that are quantised here;
-    without it they go into memory of this call's own.  It lies apart from the operands and ``out``."""
+    the operands or their scales.  A scale of x times one of w is a float32 number too: beyond 2^128 it is infinite, also where the codes
+    it scales are 0, and under 2^-126 it loses bits.  ``scratch`` (uint8, at least ``gemm_fp8_scratch_bytes(x)``) takes the codes of rows that are quantised here;
+    without it they go into memory of this call's own.  It lies apart from the operands, their scales and ``out``."""
     what = "gemm_fp8"
-    n, k, w_pitch = _codes(what, "w", w)
+    n, k, w_pitch = _code_rows(what, "w", w)
     code, to = _OPERANDS.get(x.dtype), _CODES.get(out.dtype)
     if x.dim() != 2 or code is None:
         _refuse(what, "x is a matrix of float32, bfloat16 or float8_e4m3fn")
@@ -1964,7 +1965,7 @@ def gemm_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torc
         dev = -2
     scales = s_row = s_col = 0
     if code == IE_E4M3:
-        ldx = _codes(what, "x", x)[2]
+        ldx = _code_rows(what, "x", x)[2]
         if x_scales is None or x_scales.shape != (m, kb) or x_scales.dtype is not _F32:
             _refuse(what, "codes of x come with x_scales, float32 [m, ceil(k / 128)]")
         if x_scales.get_device() != dev:

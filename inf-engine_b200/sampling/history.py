@@ -34,8 +34,8 @@ def allowed_words(allowed, vocab: int) -> np.ndarray:
 
 
 class TokenHistory:
-    """Counts and bits of every slot (``kernels.history_append`` says what they hold), and whose they are: a slot's history is that
-    of ``owner(slot)``'s first tokens, as many as were recorded."""
+    """Counts and bits of every slot (``kernels.history_append`` says what they hold), and whose they are: those of the request that was
+    written into the slot last, as far as its tokens were recorded (``current``)."""
 
     def __init__(self, rt, n_slots: int, vocab: int):
         self.rt = rt
