@@ -824,8 +824,10 @@ int launch_thin(Fp8Params p, int sms, cudaStream_t stream) {
 // Up to 16 rows of x under a weight that is not long: the weight goes from memory straight into the registers that the matrix
 // instruction reads, 16 bytes a lane, a block of K ahead of the one at work.  A warp holds 16 rows of w, the instruction's larger
 // side, and 8 NT rows of x.  The codes become halves, which hold them exactly (an instruction for e4m3 exists, but is made of the
-// same conversions, of both operands every time; they are what bounds this kernel, so slots in shared memory with more blocks of K
-// ahead do not help: 4 x 8192 x 8192 took 22 us with four, 15.9 so).  The instruction wants of lane (g, t) two numbers from 2 t and two
+// same conversions, of both operands every time).  Long weights are bound by the conversions, so slots in shared memory with more blocks
+// of K ahead do not help (4 x 8192 x 8192 took 22 us with four, 15.9 so); short ones by start and trips: 1 row under 2,048 columns takes 1.6 us
+// and the weight's bytes at 4.5 TB/s, 8 rows under 8,192 columns 5.0 us at 512 rows of w and 5.9 at 2,048, four trips of a warp one after
+// the other and the sum over 16.  The instruction wants of lane (g, t) two numbers from 2 t and two
 // from 8 + 2 t of its 16; any other dealing of K serves as well if both operands share it, so lane t takes 16 neighbouring codes of 64,
 // for four instructions.  ks warps share rows of w and deal out K where there are few rows of it; their sums come together in shared
 // memory, in the order of K.
